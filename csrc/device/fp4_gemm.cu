@@ -1,0 +1,154 @@
+// fp4_gemm.cu - products of microscaled 4-bit operands: tensor maps, choice of tile, launch (loop: fp4_gemm.cuh).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/hcomm_fp4.h"
+#include "../core/log.h"
+#include "../core/per_device.h"
+#include "fp4_gemm.cuh"
+#include "gemm_api.h"
+
+namespace {
+using namespace hcfp4;
+
+// Set when a bounded wait expired; part of the device image, so no call has to allocate it.
+__device__ uint32_t g_error;
+
+template <int BN, bool GLU>
+__global__ void __launch_bounds__(kGemmThreads, 1) Fp4GemmKernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape shape)
+{
+    GemmLoop<BN, GLU>(&maps, shape);
+}
+
+struct Device { int sms; uint32_t *error; };
+template <typename Kernel> bool AllowShared(Kernel *kernel)
+{
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess) return true;
+    cudaGetLastError();
+    return false;
+}
+bool CurrentDevice(Device *d)
+{
+    static hc::PerDevice<Device> devices;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return false; }
+    bool good = true;
+    *d = devices.Get(dev, [&](Device *v) {
+        good = cudaDeviceGetAttribute(&v->sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && cudaGetSymbolAddress((void **)&v->error, g_error) == cudaSuccess &&
+               AllowShared(Fp4GemmKernel<128, false>) && AllowShared(Fp4GemmKernel<256, false>) && AllowShared(Fp4GemmKernel<256, true>);
+        if (!good) cudaGetLastError();
+        return good;
+    });
+    return good;
+}
+
+struct Operand { const void *values, *scales; };
+
+// 128 rows x 256 columns of values; `matrices` of them one behind the other.
+HcclResult ValueMap(CUtensorMap *m, const void *values, int64_t matrices, int64_t rows, int64_t K)
+{
+    const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)rows, (uint64_t)matrices}, pitches[2] = {(uint64_t)K / 2, (uint64_t)(rows * (K / 2))};
+    const uint32_t box[3] = {128, 128, 1};
+    return hc::EncodeTensorMap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, values, 3, dims, pitches, box, true);
+}
+// Two tiles of scales that follow one another along K.
+HcclResult ScaleMap(CUtensorMap *m, const void *scales, int64_t tiles)
+{
+    const uint64_t dims[2] = {kTileBytes / 4, (uint64_t)tiles}, pitches[1] = {kTileBytes};
+    const uint32_t box[2] = {kTileBytes / 4, 2};
+    return hc::EncodeTensorMap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, 2, dims, pitches, box, false);
+}
+
+template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int smem, void *stream, const Maps &maps, const Shape &shape)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, 1, 1);
+    cfg.blockDim = dim3(kGemmThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, maps, shape);
+}
+
+// b[1] is the up projection of a gated product, else NULL.
+HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, void *out, int M, int N, int K, int64_t ldOut, const int32_t *offsets, int experts, void *stream)
+{
+    if (M < 0 || N < 0 || K < 0 || K % kBlock || ldOut < N || experts < 0 || experts > kMaxExperts || (experts > 0) != (offsets != nullptr)) {
+        RPT_ERR("EI0003", "%s: M %d, N %d, K %d (a multiple of %d), rows of the result %lld apart, %d experts (at most %d, with offsets)", what, M, N, K, kBlock, (long long)ldOut,
+                experts, kMaxExperts);
+        return HCCL_E_PARA;
+    }
+    if (M == 0 || N == 0) return HCCL_SUCCESS;
+    if (!out) return HCCL_E_PTR;
+    if ((uintptr_t)out & 1) { RPT_ERR("EI0003", "%s: misaligned result", what); return HCCL_E_PARA; }
+    if (K == 0) { RPT_ERR("EI0003", "%s: no columns to multiply", what); return HCCL_E_PARA; }
+    const Operand all[3] = {a, b[0], glu ? b[1] : b[0]};
+    for (const Operand &o : all) {
+        if (!o.values || !o.scales) return HCCL_E_PTR;
+        if (((uintptr_t)o.values & 15) || ((uintptr_t)o.scales & 15)) { RPT_ERR("EI0003", "%s: operands must be 16-byte aligned", what); return HCCL_E_PARA; }
+    }
+    Device dev;
+    if (!CurrentDevice(&dev)) { HCCL_ERROR("%s: the current device cannot run it", what); return HCCL_E_RUNTIME; }
+    Shape g = {};
+    g.M = M; g.N = N; g.K = K;
+    g.experts = experts; g.offsets = offsets;
+    g.tileCols = (K + kTileCols - 1) / kTileCols;
+    g.tileRowsB = (N + kTileRows - 1) / kTileRows;
+    g.ldOut = ldOut; g.out = (__nv_bfloat16 *)out;
+    g.error = dev.error;
+    const int matrices = std::max(experts, 1);
+    const int64_t rowTiles = experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128;
+    const bool wideTile = glu || rowTiles * ((N + 127) / 128) >= 4 * dev.sms;
+    const int bn = wideTile ? 256 : 128;
+    g.tilesN = glu ? (N + 127) / 128 : (N + bn - 1) / bn;
+    g.group = 16;
+    if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX || rowTiles * g.tileCols > INT32_MAX) {
+        RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
+        return HCCL_E_PARA;
+    }
+    Maps maps;
+    CHK_RET(ValueMap(&maps.a, a.values, 1, M, K));
+    CHK_RET(ScaleMap(&maps.sa, a.scales, rowTiles * g.tileCols));
+    for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !glu) { maps.b[1] = maps.b[0]; maps.sb[1] = maps.sb[0]; break; }
+        CHK_RET(ValueMap(&maps.b[h], b[h].values, matrices, N, K));
+        CHK_RET(ScaleMap(&maps.sb[h], b[h].scales, (int64_t)matrices * g.tileRowsB * g.tileCols));
+    }
+    const int ctas = (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);
+    cudaError_t e;
+    if (glu) e = Launch(Fp4GemmKernel<256, true>, ctas, SmemBytes<256>(experts), stream, maps, g);
+    else if (wideTile) e = Launch(Fp4GemmKernel<256, false>, ctas, SmemBytes<256>(experts), stream, maps, g);
+    else e = Launch(Fp4GemmKernel<128, false>, ctas, SmemBytes<128>(experts), stream, maps, g);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        HCCL_ERROR("%s launch failed: %s", what, cudaGetErrorString(e));
+        return HCCL_E_RUNTIME;
+    }
+    return HCCL_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" int HcommFp4Gemm(const void *aValues, const void *aScales, const void *bValues, const void *bScales, void *out, int M, int N, int K, int64_t ldOut,
+                            const int32_t *offsets, int experts, void *stream)
+{
+    return Gemm("HcommFp4Gemm", {aValues, aScales}, {{bValues, bScales}, {nullptr, nullptr}}, false, out, M, N, K, ldOut, offsets, experts, stream);
+}
+extern "C" int HcommFp4GemmSwiglu(const void *aValues, const void *aScales, const void *gValues, const void *gScales, const void *uValues, const void *uScales, void *out,
+                                  int M, int N, int K, int64_t ldOut, const int32_t *offsets, int experts, void *stream)
+{
+    return Gemm("HcommFp4GemmSwiglu", {aValues, aScales}, {{gValues, gScales}, {uValues, uScales}}, true, out, M, N, K, ldOut, offsets, experts, stream);
+}
+extern "C" int HcommFp4TakeError(void)
+{
+    uint32_t v = 0;
+    const uint32_t zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_error, sizeof(v)) != cudaSuccess) { cudaGetLastError(); return -1; }
+    if (v) cudaMemcpyToSymbol(g_error, &zero, sizeof(zero));
+    return (int)v;
+}

@@ -107,7 +107,8 @@ GemmLimits Limits()
 
 }  // namespace
 
-HcclResult MakeTensorMap2dBf16(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ldElems, uint32_t boxRows, uint32_t boxCols)
+HcclResult EncodeTensorMap(CUtensorMap *map, CUtensorMapDataType type, const void *base, int rank, const uint64_t *dims, const uint64_t *pitches, const uint32_t *box,
+                           bool swizzle)
 {
     std::call_once(g_encodeOnce, [] {
         void *fn = nullptr;
@@ -119,22 +120,26 @@ HcclResult MakeTensorMap2dBf16(CUtensorMap *map, const void *base, uint64_t rows
         HCCL_ERROR("cuTensorMapEncodeTiled is not available from this driver");
         return HCCL_E_DRV;
     }
-    if (((uintptr_t)base & 15) != 0 || (ldElems * 2) % 16 != 0) {
-        HCCL_ERROR("TMA needs a 16-byte aligned base and row pitch (base %p, pitch %llu bytes)", base, (unsigned long long)(ldElems * 2));
+    if (((uintptr_t)base & 15) != 0 || pitches[0] % 16 != 0) {
+        HCCL_ERROR("TMA needs a 16-byte aligned base and row pitch (base %p, pitch %llu bytes)", base, (unsigned long long)pitches[0]);
         return HCCL_E_PARA;
     }
-    cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ldElems * 2};
-    cuuint32_t box[2] = {boxCols, boxRows};
-    cuuint32_t elemStrides[2] = {1, 1};
-    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, elemStrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t elemStrides[3] = {1, 1, 1};
+    const cuuint64_t d[3] = {dims[0], dims[1], rank > 2 ? dims[2] : 1}, p[2] = {pitches[0], rank > 2 ? pitches[1] : 0};
+    CUresult r = g_encode(map, type, (cuuint32_t)rank, const_cast<void *>(base), d, p, box, elemStrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        HCCL_ERROR("cuTensorMapEncodeTiled failed with %d (rows %llu cols %llu ld %llu box %ux%u)", (int)r, (unsigned long long)rows,
-                   (unsigned long long)cols, (unsigned long long)ldElems, boxRows, boxCols);
+        HCCL_ERROR("cuTensorMapEncodeTiled failed with %d (rows %llu cols %llu pitch %llu bytes, box %ux%u)", (int)r, (unsigned long long)dims[1],
+                   (unsigned long long)dims[0], (unsigned long long)pitches[0], box[1], box[0]);
         return HCCL_E_DRV;
     }
     return HCCL_SUCCESS;
+}
+HcclResult MakeTensorMap2dBf16(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t ldElems, uint32_t boxRows, uint32_t boxCols)
+{
+    const uint64_t dims[2] = {cols, rows}, pitches[1] = {ldElems * 2};
+    const uint32_t box[2] = {boxCols, boxRows};
+    return EncodeTensorMap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, 2, dims, pitches, box, true);
 }
 
 // Row blocks (256 rows) per rasterisation group of the CTA-pair kernels.  The tiles in flight cover gm row blocks by

@@ -55,6 +55,33 @@ int HcommMoeTakeOverflow(void *handle);
 // race on it (not those of a single rank).  The array's address is resolved by HcommMoeCreate (set-up time); the call must be made with the
 // exchange's GPU current and is refused with HCCL_E_PARA otherwise.
 int HcommMoeDispatchStaticScratch(void *handle, const void *x, const int32_t *topkIdx, int numTokens, void *stream);
+
+/* Routing: what dispatch and combine take, from the router's logits.  No communicator is involved.
+ *
+ * logits [tokens][experts] (FP32, FP16, BFP16; rows ldLogits elements apart).  A token's k largest logits - with `bias` (f32 [experts],
+ * HCOMM_MOE_SIGMOID only): its k largest sigmoid(logit) + bias, compared in 64 bits - are its choices, largest first, of equal ones
+ * the lowest index.  p is the softmax of the logits, or the sigmoids divided by their sum.
+ *   topkIdx i32 [tokens][topk]   expert, or -1: nothing left to choose
+ *   gates   f32 [tokens][topk]   scale * score of the choice, softmax probability or sigmoid; renormalize: divided by the sum over the token's
+ *                                choices.  0 where topkIdx is -1
+ *   counts  i32 [experts + 1]    tokens that chose the expert; last: tokens counted (T)
+ *   probSums f32 [experts]       sum of p over the tokens, or NULL
+ *   loss    f32                  balance * experts * sum over e of counts[e] / (T topk) * probSums[e] / T, or NULL
+ * A logit of -inf takes the expert out for the token.  Tokens whose `valid` byte (NULL: all) is 0 choose -1, have gates of 0 and are not counted.
+ * A row that holds a NaN (or, of a softmax, +inf) chooses -1 with gates of NaN, and makes sums and loss NaN.
+ * Sums are added up in an order that depends on the sizes and the device alone.  experts <= 1024, topk <= 16.
+ * scratch: HcommMoeRouteScratchBytes, 4-byte aligned, whatever it holds; free again once the stream has passed the call. */
+#define HCOMM_MOE_SOFTMAX 0
+#define HCOMM_MOE_SIGMOID 1
+uint64_t HcommMoeRouteScratchBytes(int tokens, int experts);
+int HcommMoeRoute(const void *logits, int dataType, int64_t ldLogits, int tokens, int experts, int topk, int scoring, int renormalize, float scale, const float *bias,
+                  const uint8_t *valid, int32_t *topkIdx, float *gates, int32_t *counts, float *probSums, float balance, float *loss, void *scratch, void *stream);
+/* The loss alone, from counts and probSums that were summed over ranks. */
+int HcommMoeBalanceLoss(const int32_t *counts, const float *probSums, int experts, int topk, float balance, float *loss, void *stream);
+/* dlogits [tokens][experts] in the logits' type (rows ldGrad apart) from dgates f32 [tokens][topk] and dloss f32 (either may be NULL), with the
+ * arguments of the call in front and its topkIdx and counts (summed over ranks, where the loss was).  Rows that are not valid get 0. */
+int HcommMoeRouteBackward(const void *logits, int dataType, int64_t ldLogits, int tokens, int experts, int topk, int scoring, int renormalize, float scale, const uint8_t *valid,
+                          const int32_t *topkIdx, const float *dgates, const int32_t *counts, float balance, const float *dloss, void *dlogits, int64_t ldGrad, void *stream);
 #ifdef __cplusplus
 }
 #endif

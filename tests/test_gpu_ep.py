@@ -1,0 +1,122 @@
+"""The expert-parallel layer: routing, dispatch, 4-bit products by expert and combine in a row, each step against a plain form of the
+step in front of it, and the layer against the steps."""
+import pytest
+import torch
+
+from helpers import run_ranks
+from test_gpu_fp4 import check_gemm, gen, held, nearest, swiglu_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def make(n, **kw):
+    import hcomm_b200 as hb
+    from hcomm_b200.parallel.ep import ExpertParallelMlp
+    info = hb.get_root_info()
+    comms = run_ranks(n, lambda r: (torch.cuda.set_device(0), hb.Communicator(n, info, r, buffer_mb=8))[1])
+    layers = run_ranks(n, lambda r: (torch.cuda.set_device(0), ExpertParallelMlp(comms[r], **kw))[1])
+    return comms, layers
+
+
+def end(comms, layers):
+    run_ranks(len(comms), lambda r: (torch.cuda.set_device(0), layers[r].destroy()))
+    run_ranks(len(comms), lambda r: comms[r].destroy())
+
+
+@pytest.mark.parametrize("tokens,experts,topk,hidden,inter,scoring", [(1, 8, 2, 512, 64, "softmax"), (50, 16, 4, 512, 160, "sigmoid"), (700, 8, 2, 1024, 512, "softmax")])
+def test_each_step_of_one_rank(tokens, experts, topk, hidden, inter, scoring):
+    from hcomm_b200.ops.fp4 import gemm_fp4, gemm_fp4_swiglu, quantize_fp4
+    from hcomm_b200.ops.gemm import gemm_bf16
+    from hcomm_b200.ops.moe import quantize_e4m3_1x128
+    from hcomm_b200.ops.router import route
+    g = gen(tokens)
+    comms, (layer,) = make(1, experts=experts, topk=topk, hidden=hidden, intermediate=inter, max_tokens=tokens, scoring=scoring)
+    try:
+        x = torch.randn(tokens, hidden, device="cuda", generator=g).to(torch.bfloat16)
+        valid = torch.rand(tokens, device="cuda", generator=g) < 0.9
+        valid[0] = True
+        out = layer(x, valid=valid).clone()
+        r = layer.routing
+        assert torch.equal(route(gemm_bf16(x, layer.router), topk, scoring=scoring, valid=valid).topk_idx, r.topk_idx)
+        recv = layer.moe.dispatch(x, r.topk_idx)
+        bounds, total = recv.expert_offsets.tolist(), recv.num_rows
+        assert torch.equal(recv.expert_offsets.diff(), r.counts) and total == int(valid.sum()) * topk
+        q, s = quantize_e4m3_1x128(x)
+        tk = (recv.origin[:total] & 0xffffffff).long()
+        rows = nearest(q.float() * s.repeat_interleave(128, 1))[tk // topk]
+        h = gemm_fp4_swiglu(quantize_fp4(recv.rows, recv.scales, offsets=recv.expert_offsets), layer.gate, layer.up)
+        y = gemm_fp4(quantize_fp4(h, offsets=recv.expert_offsets), layer.down)
+        gate, up, down = held(layer.gate), held(layer.up), held(layer.down)
+        for e, (lo, hi) in enumerate(zip(bounds, bounds[1:])):
+            if lo < hi:
+                want, tol = swiglu_reference(rows[lo:hi], gate[e], up[e])
+                assert bool(((h[lo:hi].double() - want).abs() <= tol).all())
+                check_gemm(y[lo:hi], nearest(h[lo:hi]), down[e])
+        want = torch.zeros(tokens, hidden, dtype=torch.float64, device="cuda")
+        terms = r.gates.double().view(-1)[tk].unsqueeze(1) * y[:total].double()
+        want.index_add_(0, tk // topk, terms)
+        size = torch.zeros_like(want).index_add_(0, tk // topk, terms.abs())
+        # a rounding to bf16, and topk products and sums in 32 bits
+        assert bool(((out.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * topk * 2.0 ** -23).all())
+        assert (out[~valid] == 0).all()
+        # again, with the steps one by one, and in a graph: the same bits
+        assert torch.equal(layer.moe.combine(y, r.gates), out)
+        layer(x, out, valid)
+        graph, into = torch.cuda.CUDAGraph(), torch.empty_like(out)
+        with torch.cuda.graph(graph):
+            layer(x, into, valid)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(into, out)
+    finally:
+        end(comms, [layer])
+
+
+def test_two_ranks_give_what_one_gives():
+    from hcomm_b200.ops.fp4 import Fp4Tensor, quantize_fp4
+    g = gen(77)
+    experts, topk, hidden, inter, tokens = 16, 4, 512, 96, 40
+    w = {name: (torch.randn(experts, *shape, device="cuda", generator=g) * 0.05).to(torch.bfloat16)
+         for name, shape in (("w_gate", (inter, hidden)), ("w_up", (inter, hidden)), ("w_down", (hidden, inter)))}
+    router = (torch.randn(experts, hidden, device="cuda", generator=g) * 0.05).to(torch.bfloat16)
+    xs = [torch.randn(tokens, hidden, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2)]
+    options = dict(experts=experts, topk=topk, hidden=hidden, intermediate=inter, max_tokens=2 * tokens, w_router=router)
+    comms, layers = make(1, **options, **w)
+    want = layers[0](torch.cat(xs)).clone()
+    torch.cuda.synchronize()
+    end(comms, layers)
+    import hcomm_b200 as hb
+    from hcomm_b200.parallel.ep import ExpertParallelMlp
+    info = hb.get_root_info()
+    comms = run_ranks(2, lambda r: (torch.cuda.set_device(0), hb.Communicator(2, info, r, buffer_mb=8))[1])
+
+    def layer(r):
+        torch.cuda.set_device(0)
+        mine = {name: v[r * 8:r * 8 + 8] for name, v in w.items()}
+        if r == 1:                  # weights that are in 4 bits already
+            mine = {name: quantize_fp4(v) for name, v in mine.items()}
+            assert all(isinstance(v, Fp4Tensor) for v in mine.values())
+        return ExpertParallelMlp(comms[r], **options, **mine)
+    layers = run_ranks(2, layer)
+
+    def step(r):
+        torch.cuda.set_device(0)
+        out = layers[r](xs[r])
+        torch.cuda.synchronize()
+        return out
+    for _ in range(2):
+        outs = run_ranks(2, step)
+        assert torch.equal(torch.cat(outs), want)
+    assert all(x.moe.overflow() == 0 for x in layers)
+    end(comms, layers)
+
+
+def test_refusals():
+    import hcomm_b200 as hb
+    from hcomm_b200.parallel.ep import ExpertParallelMlp
+    torch.cuda.set_device(0)
+    comm = hb.Communicator(1, hb.get_root_info(), 0, buffer_mb=4)
+    for bad in (dict(experts=12), dict(w_gate=torch.zeros(8, 64, 256, device="cuda", dtype=torch.bfloat16)), dict(intermediate=48)):
+        with pytest.raises(ValueError):
+            ExpertParallelMlp(comm, **{**dict(experts=8, topk=2, hidden=512, intermediate=64, max_tokens=8), **bad})
+    comm.destroy()

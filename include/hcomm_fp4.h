@@ -36,7 +36,7 @@ uint64_t HcommFp4ScaleBytes(int64_t batch, int64_t rows, int64_t cols, int exper
  * experts > 0: offsets as above, batch 1.  1024 experts at most. */
 int HcommFp4Quantize(const void *x, int dataType, const float *xScales, int64_t batch, int64_t rows, int64_t cols, int64_t batchPitch, int64_t rowPitch,
                      int64_t scalePitch, const int32_t *offsets, int experts, void *values, void *scales, void *stream);
-/* The values that a quantised tensor stands for, contiguous, rounded to dataType (FP32, FP16, BFP16). */
+/* The values that a quantised tensor stands for, contiguous, rounded to dataType (FP32, FP16, BFP16); 32-byte aligned. */
 int HcommFp4Dequantize(const void *values, const void *scales, int64_t batch, int64_t rows, int64_t cols, const int32_t *offsets, int experts, void *out,
                        int dataType, void *stream);
 

@@ -6,21 +6,15 @@
 // function or dispatch modes, tensors of transforms): the caller then goes the general way, which also raises the errors.  A
 // failed launch comes back as its HcclResult.  Entry points are handed over as addresses, so that they are those of the library
 // that Python loaded.  The interpreter lock is released around them, since ranks of one process may wait for one another.
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/utils/pybind.h>
+#include "plain.h"
 
-#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/ops/empty.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAStream.h>
 
-#include "hccl/hccl_types.h"
 #include "released.h"
 
 namespace {
 
-using hcomm_torch::Released;
+using namespace hcomm_torch;
 using AllReduceFn = int (*)(void *, void *, uint64_t, int, int, void *, void *);
 using AllReduceScaledFn = int (*)(void *, void *, uint64_t, int, int, float, void *, void *);
 using AllGatherFn = int (*)(void *, void *, uint64_t, int, void *, void *);
@@ -28,49 +22,6 @@ using AlltoAllFn = int (*)(const void *, uint64_t, int, const void *, uint64_t, 
 using GemmFn = int (*)(const void *, const void *, void *, int, int, int, int, int, int, void *);
 using DispatchFn = int (*)(void *, const void *, const int32_t *, int, void *);
 using CombineFn = int (*)(void *, const void *, uint64_t, const float *, void *, int, void *);
-
-const c10::DispatchKeySet kPlain = c10::DispatchKeySet({c10::DispatchKey::Dense, c10::DispatchKey::AutogradFunctionality, c10::DispatchKey::ADInplaceOrView,
-                                                        c10::DispatchKey::AutocastCUDA}) |
-                                   c10::DispatchKeySet(c10::BackendComponent::CUDABit);
-
-// A strided CUDA tensor with memory of its own on the current device, nothing wrapped around it; NULL otherwise.
-const at::Tensor *Plain(PyObject *o, int device)
-{
-    if (!THPVariable_CheckExact(o)) return nullptr;
-    const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.defined()) return nullptr;
-    const c10::TensorImpl *impl = t.unsafeGetTensorImpl();
-    if ((impl->key_set().raw_repr() & ~kPlain.raw_repr()) != 0 || !t.is_cuda() || t.get_device() != device || !impl->has_storage() || impl->layout() != c10::kStrided)
-        return nullptr;
-    return &t;
-}
-bool ModesActive()
-{
-    return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-           (c10::impl::tls_local_dispatch_key_set().included_.raw_repr() & ~c10::default_included_set.raw_repr()) != 0;
-}
-// The device of this call, -1 where the general way has to be taken.
-int Device() { return ModesActive() ? -1 : (int)c10::cuda::current_device(); }
-void *StreamOf(int device) { return (void *)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
-// The address in a Python integer; false for anything else (the handle of a communicator that was destroyed is None).
-bool Address(PyObject *o, void **p)
-{
-    if (!PyLong_Check(o)) return false;
-    *p = PyLong_AsVoidPtr(o);
-    if (!PyErr_Occurred()) return true;
-    PyErr_Clear();
-    return false;
-}
-
-int TypeCode(at::ScalarType t)
-{
-    switch (t) {
-        case at::kChar: return HCCL_DATA_TYPE_INT8; case at::kShort: return HCCL_DATA_TYPE_INT16; case at::kInt: return HCCL_DATA_TYPE_INT32;
-        case at::kLong: return HCCL_DATA_TYPE_INT64; case at::kByte: return HCCL_DATA_TYPE_UINT8; case at::kFloat: return HCCL_DATA_TYPE_FP32;
-        case at::kHalf: return HCCL_DATA_TYPE_FP16; case at::kBFloat16: return HCCL_DATA_TYPE_BFP16; case at::kDouble: return HCCL_DATA_TYPE_FP64;
-        default: return -1;
-    }
-}
 
 // A matrix of bf16 whose rows are contiguous and whose sizes the entry points can take.
 bool Matrix(const at::Tensor *t)

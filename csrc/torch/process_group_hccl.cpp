@@ -547,12 +547,13 @@ c10::intrusive_ptr<c10d::Backend> CreateBackend(const c10::intrusive_ptr<c10d::S
 }
 
 bool AddNativeCalls(PyObject *module);      // native_calls.cpp
+bool AddNativeOperators(PyObject *module);  // native_operators.cpp
 
 }  // namespace hcomm_torch
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
-    if (!hcomm_torch::AddNativeCalls(m.ptr())) throw py::error_already_set();
+    if (!hcomm_torch::AddNativeCalls(m.ptr()) || !hcomm_torch::AddNativeOperators(m.ptr())) throw py::error_already_set();
     using hcomm_torch::ProcessGroupHccl;
     py::class_<ProcessGroupHccl, c10d::Backend, c10::intrusive_ptr<ProcessGroupHccl>>(m, "ProcessGroupHCCL")
         .def("allreduce_scaled", &ProcessGroupHccl::AllreduceScaled, py::arg("input"), py::arg("output"), py::arg("scale"),

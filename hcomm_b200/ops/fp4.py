@@ -19,13 +19,18 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
+from .._ext import Short
 from .._stream import raw_stream
 
 _TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16, torch.float8_e4m3fn: _lib.FP8E4M3}
 MAX_EXPERTS = 1024
 
 
-@dataclass
+_short_quantize, _short_dequantize = Short("fp4_quantize", "HcommFp4Quantize"), Short("fp4_dequantize", "HcommFp4Dequantize")
+_short_gemm, _short_swiglu = Short("fp4_gemm", "HcommFp4Gemm"), Short("fp4_gemm", "HcommFp4GemmSwiglu")
+
+
+@dataclass(slots=True)
 class Fp4Tensor:
     """A quantised matrix [rows, cols], or several of the same size [experts, rows, cols]."""
     values: torch.Tensor                    # uint8 [..., rows, cols // 2]: two values a byte, the even column in the low half
@@ -110,6 +115,9 @@ def quantize_fp4(x: torch.Tensor, scales: torch.Tensor | None = None, *, offsets
     that the expert-parallel exchange delivers; cols a multiple of 128.  With ``offsets`` (int32 [experts + 1]) rows
     offsets[e] .. offsets[e + 1] belong to expert e: the result is the left operand of a product with every expert's own matrix.
     Rows behind the last expert's are neither read nor written."""
+    r = _short_quantize(x, scales, offsets)
+    if r is not None:
+        return Fp4Tensor(r[0], r[1], offsets)
     device = _on_device("quantize_fp4", x, scales, offsets)
     fp8 = x.dtype == torch.float8_e4m3fn
     if x.dtype not in _TYPES or fp8 != (scales is not None):
@@ -143,6 +151,9 @@ def quantize_fp4(x: torch.Tensor, scales: torch.Tensor | None = None, *, offsets
 
 def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, in bf16 (exact unless tiny), fp16 or fp32.  Rows behind the last expert's are left undefined."""
+    r = _short_dequantize(q.values, q.scales, q.offsets, _TYPES.get(dtype, -1)) if q.__class__ is Fp4Tensor else None
+    if r is not None:
+        return r
     device = _check_operand("dequantize_fp4", q)
     if dtype not in _TYPES or dtype == torch.float8_e4m3fn:
         raise TypeError("dequantize_fp4 makes fp32, fp16 or bf16")
@@ -210,11 +221,19 @@ def gemm_fp4(a: Fp4Tensor, b: Fp4Tensor, out: torch.Tensor | None = None) -> tor
 
     Of rows grouped by expert and b [experts, N, K], each row with its expert's matrix; rows of ``out`` behind the last expert's are
     left as they were."""
+    if a.__class__ is Fp4Tensor and b.__class__ is Fp4Tensor and b.offsets is None:
+        r = _short_gemm(a.values, a.scales, a.offsets, out, b.values, b.scales)
+        if r is not None:
+            return r
     return _multiply("HcommFp4Gemm", "gemm_fp4", a, (b,), out)
 
 
 def gemm_fp4_swiglu(a: Fp4Tensor, gate: Fp4Tensor, up: Fp4Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """``silu(a @ gate.T) * (a @ up.T)``, bf16, from the fp32 accumulators of both; rows grouped by expert as in ``gemm_fp4``."""
+    if a.__class__ is gate.__class__ is up.__class__ is Fp4Tensor and gate.offsets is up.offsets is None:
+        r = _short_swiglu(a.values, a.scales, a.offsets, out, gate.values, gate.scales, up.values, up.scales)
+        if r is not None:
+            return r
     return _multiply("HcommFp4GemmSwiglu", "gemm_fp4_swiglu", a, (gate, up), out)
 
 

@@ -19,12 +19,27 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from .._ext import Short, entry
 from .._stream import raw_stream
 from ..comm import Communicator
 
 SCORINGS = {"softmax": 0, "sigmoid": 1}
 _TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 MAX_EXPERTS, MAX_TOPK = 1024, 16
+
+
+class _ShortRoute(Short):
+    """The native call, which is given the entry points of the backward pass and of the scratch's size as well."""
+
+    __slots__ = ("_others",)
+
+    def __call__(self, *args):
+        if self._call is None and self.find() is not None:
+            self._others = entry("HcommMoeRouteBackward"), entry("HcommMoeRouteScratchBytes")
+        return super().__call__(*self._others, *args)
+
+
+_short_route = _ShortRoute("moe_route", "HcommMoeRoute")
 
 
 class Routing(NamedTuple):
@@ -123,6 +138,10 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", renormal
                  the one loss with regard to its own logits
 
     A logit of -inf takes the expert out for the token.  A row that holds a NaN (under softmax: or +inf) chooses -1 with gates of NaN."""
+    if comm is None and topk.__class__ is int and scoring in SCORINGS:
+        r = _short_route(logits, topk, SCORINGS[scoring], 1 if renormalize else 0, float(scale), bias, valid, float(balance))
+        if r is not None:
+            return Routing(*r)
     if scoring not in SCORINGS:
         raise ValueError(f"scoring must be one of {sorted(SCORINGS)}")
     if logits.dim() != 2 or logits.dtype not in _TYPES:

@@ -18,7 +18,8 @@ __host__ __device__ constexpr uint32_t ScaleByte(uint32_t r) { return (r % 32) *
 
 // Where the rows of each expert start, and its tiles of scales, from the offsets in device memory.  Offsets are clamped to
 // [0, rows] and made to rise, so that whatever they hold, rows and tiles stay inside their buffers:
-// sum of ceil(rows of e / 128) <= GroupedTileRows.  One warp calls it; start and tile have experts + 1 entries in shared memory.
+// sum of ceil(rows of e / 128) <= GroupedTileRows.  One warp calls it; start and, where it is wanted, tile have experts + 1
+// entries in shared memory.
 __device__ __forceinline__ void BuildGroups(const int32_t *offsets, int experts, int rows, int *start, int *tile)
 {
     const int lane = threadIdx.x & 31;
@@ -42,7 +43,10 @@ __device__ __forceinline__ void BuildGroups(const int32_t *offsets, int experts,
             if (lane >= d) t += o;
         }
         t += before;
-        if (e <= experts) { start[e] = v; tile[e] = t; }
+        if (e <= experts) {
+            start[e] = v;
+            if (tile) tile[e] = t;
+        }
         low = last = __shfl_sync(0xffffffffu, v, 31);
         before = __shfl_sync(0xffffffffu, t, 31);
     }

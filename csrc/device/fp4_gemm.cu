@@ -8,6 +8,7 @@
 #include "../core/log.h"
 #include "../core/per_device.h"
 #include "fp4_gemm.cuh"
+#include "fp4_gemm_pair.cuh"
 #include "gemm_api.h"
 
 namespace {
@@ -22,12 +23,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1) Fp4GemmKernel(const __grid_co
     GemmLoop<BN, GLU>(&maps, shape);
 }
 
-struct Device { int sms; uint32_t *error; };
+template <bool GLU>
+__global__ void __launch_bounds__(kGemmThreads, 1) Fp4GemmPairKernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape shape)
+{
+    GemmLoopPair<GLU>(&maps, shape);
+}
+
+struct Device { int sms, pairs; uint32_t *error; };          // pairs: clusters of two CTAs that fit at once
 template <typename Kernel> bool AllowShared(Kernel *kernel)
 {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess) return true;
     cudaGetLastError();
     return false;
+}
+cudaLaunchConfig_t Config(cudaLaunchAttribute *at, int ctas, int clusterCtas, int smem, void *stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, 1, 1);
+    cfg.blockDim = dim3(kGemmThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = clusterCtas; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = clusterCtas > 1 ? 2 : 1;
+    return cfg;
 }
 bool CurrentDevice(Device *d)
 {
@@ -37,7 +58,11 @@ bool CurrentDevice(Device *d)
     bool good = true;
     *d = devices.Get(dev, [&](Device *v) {
         good = cudaDeviceGetAttribute(&v->sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && cudaGetSymbolAddress((void **)&v->error, g_error) == cudaSuccess &&
-               AllowShared(Fp4GemmKernel<128, false>) && AllowShared(Fp4GemmKernel<256, false>) && AllowShared(Fp4GemmKernel<256, true>);
+               AllowShared(Fp4GemmKernel<128, false>) && AllowShared(Fp4GemmKernel<256, false>) && AllowShared(Fp4GemmKernel<256, true>) &&
+               AllowShared(Fp4GemmPairKernel<false>) && AllowShared(Fp4GemmPairKernel<true>);
+        cudaLaunchAttribute at[2];
+        const cudaLaunchConfig_t cfg = Config(at, v->sms / 2 * 2, 2, PairSmemBytes(kMaxExperts), nullptr);
+        good = good && cudaOccupancyMaxActiveClusters(&v->pairs, Fp4GemmPairKernel<true>, &cfg) == cudaSuccess;
         if (!good) cudaGetLastError();
         return good;
     });
@@ -61,17 +86,10 @@ HcclResult ScaleMap(CUtensorMap *m, const void *scales, int64_t tiles)
     return hc::EncodeTensorMap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, 2, dims, pitches, box, false);
 }
 
-template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int smem, void *stream, const Maps &maps, const Shape &shape)
+template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clusterCtas, int smem, void *stream, const Maps &maps, const Shape &shape)
 {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, 1, 1);
-    cfg.blockDim = dim3(kGemmThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2];
+    const cudaLaunchConfig_t cfg = Config(at, ctas, clusterCtas, smem, stream);
     return cudaLaunchKernelEx(&cfg, kernel, maps, shape);
 }
 
@@ -103,10 +121,13 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     g.error = dev.error;
     const int matrices = std::max(experts, 1);
     const int64_t rowTiles = experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128;
-    const bool wideTile = glu || rowTiles * ((N + 127) / 128) >= 4 * dev.sms;
-    const int bn = wideTile ? 256 : 128;
-    g.tilesN = glu ? (N + 127) / 128 : (N + bn - 1) / bn;
-    g.group = 16;
+    const int64_t columns = glu ? (N + 127) / 128 : (N + 255) / 256;
+    // Rows of A by the tile: all there may be, or as many as an expert has on average (how many it has is known on the device only).
+    const int64_t pairTiles = experts > 0 ? (M + 255) / 256 + std::min(M, experts) / 2 : (M + 255) / 256;
+    const bool pairs = dev.pairs > 0 && pairTiles * columns >= dev.pairs && (experts == 0 ? M > 128 : M >= 128 * experts);
+    const bool wideTile = pairs || glu || rowTiles * ((N + 127) / 128) >= 4 * dev.sms;
+    g.tilesN = wideTile ? (int)columns : (N + 127) / 128;
+    g.group = pairs ? 8 : 16;
     if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX || rowTiles * g.tileCols > INT32_MAX) {
         RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
         return HCCL_E_PARA;
@@ -121,9 +142,12 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     }
     const int ctas = (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);
     cudaError_t e;
-    if (glu) e = Launch(Fp4GemmKernel<256, true>, ctas, SmemBytes<256>(experts), stream, maps, g);
-    else if (wideTile) e = Launch(Fp4GemmKernel<256, false>, ctas, SmemBytes<256>(experts), stream, maps, g);
-    else e = Launch(Fp4GemmKernel<128, false>, ctas, SmemBytes<128>(experts), stream, maps, g);
+    if (pairs) {
+        const int both = 2 * (int)std::min<int64_t>(dev.pairs, (experts > 0 ? rowTiles : pairTiles) * g.tilesN);
+        e = glu ? Launch(Fp4GemmPairKernel<true>, both, 2, PairSmemBytes(experts), stream, maps, g) : Launch(Fp4GemmPairKernel<false>, both, 2, PairSmemBytes(experts), stream, maps, g);
+    } else if (glu) e = Launch(Fp4GemmKernel<256, true>, ctas, 1, SmemBytes<256>(experts), stream, maps, g);
+    else if (wideTile) e = Launch(Fp4GemmKernel<256, false>, ctas, 1, SmemBytes<256>(experts), stream, maps, g);
+    else e = Launch(Fp4GemmKernel<128, false>, ctas, 1, SmemBytes<128>(experts), stream, maps, g);
     if (e != cudaSuccess) {
         cudaGetLastError();
         HCCL_ERROR("%s launch failed: %s", what, cudaGetErrorString(e));

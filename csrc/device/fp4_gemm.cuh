@@ -10,7 +10,8 @@
 // Warp roles:
 //   warp 0      TMA producer: 256 columns a stage - rows of A and B (128-byte swizzle) and their tiles of scales
 //   warp 1      issuer: copies a stage's scales to tensor memory, then four products of 64 columns; one thread
-//   warps 4-7   epilogue: accumulator rows to bf16, through shared memory, out in whole segments of the result's rows
+//   warps 4-11  epilogue: first the whole accumulator as bf16 into registers, which hands it back to the issuer after a few hundred
+//               cycles, then through shared memory out in whole segments of the result's rows
 // Each stage of the ring has its own columns for scales in tensor memory, so that the barrier that frees the stage frees them too.
 //
 // Rows of A may be grouped by expert, with a matrix of B for each: tiles never cross a group; what a tile loads behind its
@@ -29,7 +30,8 @@ using namespace sm100;
 
 constexpr int kStageCols = 256;             // columns of K a stage, 128 bytes
 constexpr int kUmmaCols = 64;               // of an instruction
-constexpr int kGemmThreads = 256;
+constexpr int kStoreWarps = 8;                        // of the epilogue: two for each quarter of the accumulator's rows
+constexpr int kGemmThreads = 32 * (4 + kStoreWarps);
 constexpr int kSlabCols = 32;               // columns that an epilogue warp stages at a time
 constexpr int kSlabBytes = 32 * kSlabCols * 2;
 
@@ -64,10 +66,10 @@ struct State {
     uint32_t tmem;
     volatile uint32_t abort;
 };
-// Behind the ring: the epilogue's slabs, the barriers, and with grouped rows two tables.
+// Behind the ring: the epilogue's slabs, the barriers, and with grouped rows where they start.
 template <int BN> constexpr int SmemBytes(int experts)
 {
-    return 1024 + Config<BN>::kStages * Config<BN>::kStageBytes + 4 * kSlabBytes + 256 + (experts > 0 ? 2 * 4 * (experts + 1) : 0);
+    return 1024 + Config<BN>::kStages * Config<BN>::kStageBytes + kStoreWarps * kSlabBytes + 256 + (experts > 0 ? 4 * (experts + 1) : 0);
 }
 
 // kind::mxf4: e2m1 x e2m1 with scales that are powers of two, both operands with K contiguous.  The fields of the scales' byte
@@ -100,32 +102,39 @@ __device__ __forceinline__ void TmaLoad3d(void *dst, const CUtensorMap *m, uint6
 }
 
 struct Tile {
-    int expert, row, rows;      // first row, rows up to the end of the group (at most 128)
+    int expert, row, rows;      // first row, rows up to the end of the group (at most 128; none or fewer: nothing to store)
     int column;                 // tile along N
     int scaleTile;              // tile row of A's scales
 };
-// The tiles that a CTA takes, t, t + step, ...: experts in order, inside an expert `group` row tiles by all columns of tiles, so
-// that CTAs that run at the same time share rows of both operands in L2.
-struct Tiles {
+// The tiles of ROWS rows that a CTA (or pair, of which `half` is the CTA) takes, t, t + step, ...: experts in order, inside an expert
+// `group` row tiles by all columns of tiles, so that CTAs that run at the same time share rows of both operands in L2.
+template <int ROWS> struct Tiles {
     const Shape &g;
-    const int *start, *tile;    // shared memory, with grouped rows
-    int expert = 0, t;
-    __device__ Tiles(const Shape &s, const int *st, const int *ti) : g(s), start(st), tile(ti), t(blockIdx.x) {}
+    const int *start;           // shared memory, with grouped rows
+    int half, step, t, expert = 0, before = 0, scalesBefore = 0;        // before: tiles of ROWS rows (tile rows of scales) of the experts in front
+    __device__ Tiles(const Shape &s, const int *st, int first, int stride, int h) : g(s), start(st), half(h), step(stride), t(first) {}
     __device__ bool Next(Tile *out)
     {
-        int firstTile = 0, firstRow = 0, endRow = g.M;
+        int firstRow = 0, endRow = g.M, rowTiles;
         if (g.experts > 0) {
-            while (expert < g.experts && t >= tile[expert + 1] * g.tilesN) ++expert;
-            if (expert == g.experts) return false;
-            firstTile = tile[expert]; firstRow = start[expert]; endRow = start[expert + 1];
-        } else if (t >= (g.M + 127) / 128 * g.tilesN) return false;
-        const int rowTiles = (endRow - firstRow + 127) / 128, local = t - firstTile * g.tilesN;
-        const int perGroup = g.group * g.tilesN, group = local / perGroup, in = local - group * perGroup;
+            for (;; ++expert) {
+                if (expert == g.experts) return false;
+                firstRow = start[expert]; endRow = start[expert + 1];
+                rowTiles = (endRow - firstRow + ROWS - 1) / ROWS;
+                if (t < (before + rowTiles) * g.tilesN) break;
+                before += rowTiles;
+                scalesBefore += (endRow - firstRow + kTileRows - 1) / kTileRows;
+            }
+        } else {
+            rowTiles = (endRow + ROWS - 1) / ROWS;
+            if (t >= rowTiles * g.tilesN) return false;
+        }
+        const int local = t - before * g.tilesN, perGroup = g.group * g.tilesN, group = local / perGroup, in = local - group * perGroup;
         const int wide = min(g.group, rowTiles - group * g.group);
         const int column = in / wide, r = group * g.group + in - column * wide;
-        out->expert = expert; out->column = column; out->scaleTile = firstTile + r;
-        out->row = firstRow + r * 128; out->rows = min(128, endRow - out->row);
-        t += gridDim.x;
+        out->expert = expert; out->column = column; out->scaleTile = scalesBefore + r * (ROWS / kTileRows) + half;
+        out->row = firstRow + r * ROWS + half * 128; out->rows = min(128, endRow - out->row);
+        t += step;
         return true;
     }
 };
@@ -161,6 +170,48 @@ __device__ __forceinline__ void StoreSlab(uint8_t *slab, const uint32_t (&packed
     __syncwarp();
 }
 
+// A warp's 32 rows and half of the columns of a finished accumulator.  handBack is called once they are in registers: the next
+// tile's products start while these are on their way out (8192 x 28672 x 8192 by pairs of CTAs: BEFORE us with it at the end, AFTER so).
+template <int BN, bool GLU, typename HandBack>
+__device__ __forceinline__ void StoreTile(const Shape &g, const Tile &t, uint32_t accumulator, int warp, int lane, uint8_t *slab, bool wide, HandBack handBack)
+{
+    constexpr int kOut = GLU ? BN / 2 : BN, kMine = kOut / 2, kSlabs = kMine / kSlabCols;
+    const int q = warp & 3, first = (warp >> 2) * kMine;
+    const int rows = t.rows - q * 32, cols = g.N - t.column * kOut - first;
+    uint32_t packed[kSlabs][16];
+    if (rows > 0) {
+        const uint32_t from = accumulator + ((uint32_t)(q * 32) << 16) + first;
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c) {
+            uint32_t v[32];
+            TmemLoad32x32(from + c * kSlabCols, v);
+            if constexpr (GLU) {
+                uint32_t u[32];
+                TmemLoad32x32(from + kOut + c * kSlabCols, u);
+                TmemLoadWait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    packed[c][j] = Bf16Pair(SiluTimes(__uint_as_float(v[2 * j]), __uint_as_float(u[2 * j])), SiluTimes(__uint_as_float(v[2 * j + 1]), __uint_as_float(u[2 * j + 1])));
+            } else {
+                TmemLoadWait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) packed[c][j] = Bf16Pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            }
+        }
+    }
+    TcFenceBefore();
+    __syncwarp();
+    if (lane == 0) handBack();
+    if (rows > 0) {
+        __nv_bfloat16 *out = g.out + (int64_t)(t.row + q * 32) * g.ldOut + t.column * kOut + first;
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+            if (c * kSlabCols < cols) StoreSlab(slab, packed[c], lane, rows, out + c * kSlabCols, g.ldOut, cols - c * kSlabCols, wide);
+    }
+}
+
+static_assert(SmemBytes<128>(kMaxExperts) <= 227 * 1024 && SmemBytes<256>(kMaxExperts) <= 227 * 1024, "shared memory");
+
 template <int BN, bool GLU>
 __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
 {
@@ -169,15 +220,15 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
     extern __shared__ uint8_t smemRaw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
     uint8_t *slabs = smem + Cfg::kStages * Cfg::kStageBytes;
-    State *st = (State *)(slabs + 4 * kSlabBytes);
+    State *st = (State *)(slabs + kStoreWarps * kSlabBytes);
     static_assert(sizeof(State) <= 256, "barriers");
-    int *start = (int *)((uint8_t *)st + 256), *tile = start + g.experts + 1;
+    int *start = (int *)((uint8_t *)st + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int stages = (g.K + kStageCols - 1) / kStageCols;
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) { MbarInit(&st->full[s], 1); MbarInit(&st->empty[s], 1); }
-        for (int a = 0; a < 2; ++a) { MbarInit(&st->accFull[a], 1); MbarInit(&st->accEmpty[a], 4); }
+        for (int a = 0; a < 2; ++a) { MbarInit(&st->accFull[a], 1); MbarInit(&st->accEmpty[a], kStoreWarps); }
         st->abort = 0;
         MbarFenceInit();
         TmaPrefetchDescriptor(&maps->a); TmaPrefetchDescriptor(&maps->b[0]);
@@ -188,7 +239,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
     }
     if (g.experts > 0 && warp == 2) {
         GridDependencyWait();
-        BuildGroups(g.offsets, g.experts, g.M, start, tile);
+        BuildGroups(g.offsets, g.experts, g.M, start, nullptr);
     }
     TcFenceBefore();
     __syncthreads();
@@ -202,7 +253,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
             GridDependencyWait();
             uint32_t it = 0;
             bool alive = true;
-            Tiles tiles(g, start, tile);
+            Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
                 const int n = t.column * (GLU ? 128 : BN);
@@ -229,7 +280,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
             GridDependencyWait();
             uint32_t it = 0, i = 0;
             bool alive = true;
-            Tiles tiles(g, start, tile);
+            Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
                 const uint32_t acc = i % Cfg::kAccumulators, phase = (i / Cfg::kAccumulators) & 1;
@@ -266,11 +317,10 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
     } else if (warp >= 4) {
         // ------------------------------------------------------------------------------------ epilogue
         GridDependencyWait();
-        const int q = warp & 3;
-        uint8_t *slab = slabs + q * kSlabBytes;
+        uint8_t *slab = slabs + (warp - 4) * kSlabBytes;
         const bool wide = g.ldOut % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
         uint32_t i = 0;
-        Tiles tiles(g, start, tile);
+        Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
         Tile t;
         while (tiles.Next(&t)) {
             const uint32_t acc = i % Cfg::kAccumulators, phase = (i / Cfg::kAccumulators) & 1;
@@ -278,33 +328,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
             if (!MbarWait(&st->accFull[acc], phase, &st->abort)) break;
             __syncwarp();
             TcFenceAfter();
-            constexpr int kOut = GLU ? 128 : BN;
-            const int rows = t.rows - q * 32, cols = g.N - t.column * kOut;
-            __nv_bfloat16 *out = g.out + (int64_t)(t.row + q * 32) * g.ldOut + t.column * kOut;
-            if (rows > 0) {
-                const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
-#pragma unroll 1
-                for (int c = 0; c < kOut && c < cols; c += kSlabCols) {
-                    uint32_t v[32], packed[16];
-                    TmemLoad32x32(from + c, v);
-                    if constexpr (GLU) {
-                        uint32_t u[32];
-                        TmemLoad32x32(from + 128 + c, u);
-                        TmemLoadWait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            packed[j] = Bf16Pair(SiluTimes(__uint_as_float(v[2 * j]), __uint_as_float(u[2 * j])), SiluTimes(__uint_as_float(v[2 * j + 1]), __uint_as_float(u[2 * j + 1])));
-                    } else {
-                        TmemLoadWait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) packed[j] = Bf16Pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                    }
-                    StoreSlab(slab, packed, lane, rows, out + c, g.ldOut, cols - c, wide);
-                }
-            }
-            TcFenceBefore();
-            __syncwarp();
-            if (lane == 0) MbarArrive(&st->accEmpty[acc]);
+            StoreTile<BN, GLU>(g, t, tmem + acc * BN, warp - 4, lane, slab, wide, [&] { MbarArrive(&st->accEmpty[acc]); });
         }
     }
     // ---------------------------------------------------------------------------------------- the end

@@ -1,0 +1,176 @@
+// fp4_gemm_pair.cuh - the loop of fp4_gemm.cuh on pairs of CTAs (cta_group::2), for many rows.
+//
+// Two CTAs of a cluster make one tile of 256 rows x 256 columns: each loads 128 rows of A and 128 rows of B, half of what
+// 128 x 256 tiles of lone CTAs load for as many products - which is what bounds those: 52 KB a stage of 512 cycles, where L2 delivers
+// some 55 bytes a cycle and SM.  The tensor core of each SM reads the other half of B from its neighbour's shared memory.
+//   * every load of a stage completes on the leader's "full" barrier; the leader's issuer alone copies scales and multiplies,
+//     for both (each CTA's scales come from its own shared memory into its own tensor memory);
+//   * scales of B are wanted whole in both CTAs, so each loads all of them;
+//   * a commit with a mask of both CTAs frees a stage, or publishes the accumulator, on either side.
+// A gated product has gate's 128 rows in the leader and up's in the other CTA.
+#pragma once
+#include "fp4_gemm.cuh"
+#include "gemm_sm100_2sm.cuh"
+
+namespace hcfp4 {
+
+template <int STAGES> struct PairConfig {
+    static constexpr int kStages = STAGES;
+    static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128, kSaBytes = 2 * kTileBytes, kSbBytes = 2 * 2 * kTileBytes;
+    static constexpr int kStageBytes = kABytes + kBBytes + kSaBytes + kSbBytes;
+    static constexpr int kScaleCols = 24, kScaleBase = 256;
+    static_assert(kScaleBase + STAGES * kScaleCols <= 512, "tensor memory");
+};
+constexpr int kPairStages = 5;
+constexpr int PairSmemBytes(int experts)
+{
+    return 1024 + kPairStages * PairConfig<kPairStages>::kStageBytes + kStoreWarps * kSlabBytes + 256 + (experts > 0 ? 4 * (experts + 1) : 0);
+}
+
+__device__ __forceinline__ void CopyScalesPair(uint32_t tmem, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void MmaMxf4Pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void TmaLoad3dPair(void *dst, const CUtensorMap *m, uint32_t bar, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(SmemAddr(dst)), "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+template <bool GLU> __device__ __forceinline__ void GemmLoopPair(const Maps *maps, const Shape &g)
+{
+    using Cfg = PairConfig<kPairStages>;
+    using namespace hcgemm::pair;
+    extern __shared__ uint8_t smemRaw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
+    uint8_t *slabs = smem + Cfg::kStages * Cfg::kStageBytes;
+    State *st = (State *)(slabs + kStoreWarps * kSlabBytes);
+    int *start = (int *)((uint8_t *)st + 256);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)ClusterCtaRank(), first = (int)ClusterId(), step = (int)NumClusters();
+    const bool leader = rank == 0;
+    const int stages = (g.K + kStageCols - 1) / kStageCols;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::kStages; ++s) { MbarInit(&st->full[s], 1); MbarInit(&st->empty[s], 1); }
+        MbarInit(&st->accFull[0], 1); MbarInit(&st->accEmpty[0], 2 * kStoreWarps);          // the epilogue warps of both CTAs
+        st->abort = 0;
+        MbarFenceInit();
+        TmaPrefetchDescriptor(&maps->a); TmaPrefetchDescriptor(&maps->b[0]);
+    }
+    if (warp == 1) {
+        TmemAlloc2(&st->tmem, 512);
+        TmemRelinquish2();
+    }
+    if (g.experts > 0 && warp == 2) {
+        GridDependencyWait();
+        BuildGroups(g.offsets, g.experts, g.M, start, nullptr);
+    }
+    TcFenceBefore();
+    __syncthreads();
+    ClusterSync();          // the other CTA's barriers are there before anything signals them
+    TcFenceAfter();
+    const uint32_t tmem = st->tmem;
+    GridDependentsLaunch();
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer (both CTAs)
+        if (ElectOne()) {
+            GridDependencyWait();
+            uint32_t it = 0;
+            bool alive = true;
+            Tiles<256> tiles(g, start, first, step, rank);
+            Tile t;
+            while (alive && tiles.Next(&t)) {
+                const int n = t.column * (GLU ? 128 : 256);
+                const int mine = GLU ? n : n + rank * 128;           // this CTA's rows of B
+                for (int k = 0; k < stages; ++k, ++it) {
+                    const int s = it % Cfg::kStages;
+                    if (!MbarWait(&st->empty[s], ((it / Cfg::kStages) & 1) ^ 1, &st->abort)) { alive = false; break; }
+                    uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
+                    if (leader) MbarExpectTx(&st->full[s], 2 * Cfg::kStageBytes);
+                    const uint32_t bar = MapToCta(&st->full[s], 0);
+                    TmaLoad3dPair(a, &maps->a, bar, k * 128, t.row, 0);
+                    TmaLoad3dPair(b, GLU && !leader ? &maps->b[1] : &maps->b[0], bar, k * 128, mine, t.expert);
+                    TmaLoad2dPair(sa, &maps->sa, bar, 0, t.scaleTile * g.tileCols + 2 * k);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        TmaLoad2dPair(sb + h * 2 * kTileBytes, &maps->sb[GLU ? h : 0], bar, 0,
+                                      (t.expert * g.tileRowsB + n / 128 + (GLU ? 0 : h)) * g.tileCols + 2 * k);
+                }
+            }
+            if (!alive) __nanosleep(500000);        // copies under way still write here: they end long before this does
+        }
+    } else if (warp == 1) {
+        // -------------------------------------------------------------------- issuer (leader CTA only)
+        if (leader && ElectOne()) {
+            GridDependencyWait();
+            uint32_t it = 0, i = 0;
+            bool alive = true;
+            Tiles<256> tiles(g, start, first, step, rank);
+            Tile t;
+            while (alive && tiles.Next(&t)) {
+                if (!MbarWait(&st->accEmpty[0], (i & 1) ^ 1, &st->abort)) { alive = false; break; }
+                ++i;
+                TcFenceAfter();
+                for (int k = 0; k < stages; ++k, ++it) {
+                    const int s = it % Cfg::kStages;
+                    if (!MbarWait(&st->full[s], (it / Cfg::kStages) & 1, &st->abort)) { alive = false; break; }
+                    TcFenceAfter();
+                    uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
+                    const uint32_t ta = tmem + Cfg::kScaleBase + s * Cfg::kScaleCols, tb = ta + 8;
+                    const int left = g.K - k * kStageCols;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (c * kTileCols >= left) break;
+                        CopyScalesPair(ta + c * 4, ScaleDesc(sa + c * kTileBytes));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) CopyScalesPair(tb + c * 8 + h * 4, ScaleDesc(sb + (h * 2 + c) * kTileBytes));
+                    }
+                    const uint64_t da = SmemDescKMajorSw128(a), db = SmemDescKMajorSw128(b);
+#pragma unroll
+                    for (int u = 0; u < kStageCols / kUmmaCols; ++u) {
+                        if (u * kUmmaCols >= left) break;
+                        MmaMxf4Pair(tmem, da + u * 2, db + u * 2, InstrDescMxf4(256, 256, (u & 1) * 2), ta + (u >> 1) * 4, tb + (u >> 1) * 8, (k | u) != 0);
+                    }
+                    MmaCommitPair(&st->empty[s]);
+                }
+                if (alive) MmaCommitPair(&st->accFull[0]);
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------------------------------------------------------------- epilogue (both CTAs)
+        GridDependencyWait();
+        uint8_t *slab = slabs + (warp - 4) * kSlabBytes;
+        const bool wide = g.ldOut % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
+        uint32_t i = 0;
+        Tiles<256> tiles(g, start, first, step, rank);
+        Tile t;
+        while (tiles.Next(&t)) {
+            if (!MbarWait(&st->accFull[0], i & 1, &st->abort)) break;
+            ++i;
+            __syncwarp();
+            TcFenceAfter();
+            StoreTile<256, GLU>(g, t, tmem, warp - 4, lane, slab, wide, [&] {
+                if (leader) MbarArrive(&st->accEmpty[0]);
+                else RemoteArrive(MapToCta(&st->accEmpty[0], 0));
+            });
+        }
+    }
+    // Nobody leaves while the other CTA may still read this one's shared memory or signal its barriers, also after a wait that ran out.
+    TcFenceBefore();
+    __syncthreads();
+    ClusterSync();
+    if (warp == 1) TmemDealloc2(tmem, 512);
+    if (threadIdx.x == 0 && st->abort) atomicExch(g.error, 1u);
+}
+
+}  // namespace hcfp4

@@ -71,11 +71,11 @@ bool CurrentDevice(Device *d)
 
 struct Operand { const void *values, *scales; };
 
-// 128 rows x 256 columns of values; `matrices` of them one behind the other.
-HcclResult ValueMap(CUtensorMap *m, const void *values, int64_t matrices, int64_t rows, int64_t K)
+// boxRows rows x 256 columns of values; `matrices` of them one behind the other.
+HcclResult ValueMap(CUtensorMap *m, const void *values, int64_t matrices, int64_t rows, int64_t K, int boxRows)
 {
     const uint64_t dims[3] = {(uint64_t)K / 2, (uint64_t)rows, (uint64_t)matrices}, pitches[2] = {(uint64_t)K / 2, (uint64_t)(rows * (K / 2))};
-    const uint32_t box[3] = {128, 128, 1};
+    const uint32_t box[3] = {128, (uint32_t)boxRows, 1};
     return hc::EncodeTensorMap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, values, 3, dims, pitches, box, true);
 }
 // Two tiles of scales that follow one another along K.
@@ -132,12 +132,20 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
         RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
         return HCCL_E_PARA;
     }
+    // A SM's loads take some 55 bytes a cycle, rows outside the matrix as long as others: 16 x 18944 x 8192 with boxes of 128 rows
+    // BOX128 us, of 16 BOX16.  Rows of an expert, which are known on the device only, come in boxes of 32 where there are few of them.
+    g.boxRows = 128;
+    if (!pairs) {
+        const int likely = experts > 0 ? M / experts : M;
+        while (g.boxRows > 8 && g.boxRows / 2 >= likely) g.boxRows /= 2;
+        if (experts > 0) g.boxRows = likely >= 96 ? 128 : 32;
+    }
     Maps maps;
-    CHK_RET(ValueMap(&maps.a, a.values, 1, M, K));
+    CHK_RET(ValueMap(&maps.a, a.values, 1, M, K, g.boxRows));
     CHK_RET(ScaleMap(&maps.sa, a.scales, rowTiles * g.tileCols));
     for (int h = 0; h < 2; ++h) {
         if (h == 1 && !glu) { maps.b[1] = maps.b[0]; maps.sb[1] = maps.sb[0]; break; }
-        CHK_RET(ValueMap(&maps.b[h], b[h].values, matrices, N, K));
+        CHK_RET(ValueMap(&maps.b[h], b[h].values, matrices, N, K, 128));
         CHK_RET(ScaleMap(&maps.sb[h], b[h].scales, (int64_t)matrices * g.tileRowsB * g.tileCols));
     }
     const int ctas = (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);

@@ -41,6 +41,7 @@ struct Shape {
     int M, N, K;
     int tilesN;
     int group;                  // row tiles that are taken together before the next column of tiles
+    int boxRows;                // rows of A that a load takes: a tile loads no more than it needs (one CTA a tile)
     int experts;                // 0: one matrix
     const int32_t *offsets;
     int tileCols, tileRowsB;    // tiles of scales along K; along N of one matrix
@@ -257,12 +258,14 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
             Tile t;
             while (alive && tiles.Next(&t)) {
                 const int n = t.column * (GLU ? 128 : BN);
+                const int boxes = (t.rows + g.boxRows - 1) / g.boxRows, bytes = Cfg::kStageBytes - Cfg::kABytes + boxes * g.boxRows * 128;
                 for (int k = 0; k < stages; ++k, ++it) {
                     const int s = it % Cfg::kStages;
                     if (!MbarWait(&st->empty[s], ((it / Cfg::kStages) & 1) ^ 1, &st->abort)) { alive = false; break; }
                     uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
-                    MbarExpectTx(&st->full[s], Cfg::kStageBytes);
-                    TmaLoad3d(a, &maps->a, &st->full[s], k * 128, t.row, 0);          // coordinates as many as the map has dimensions
+                    MbarExpectTx(&st->full[s], bytes);
+                    // as many coordinates as the map has dimensions; rows that are not loaded hold what was there, and are not stored
+                    for (int r = 0; r < boxes; ++r) TmaLoad3d(a + r * g.boxRows * 128, &maps->a, &st->full[s], k * 128, t.row + r * g.boxRows, 0);
                     TmaLoad2d(sa, &maps->sa, &st->full[s], 0, t.scaleTile * g.tileCols + 2 * k);
 #pragma unroll
                     for (int h = 0; h < BN / 128; ++h) {

@@ -17,10 +17,10 @@ using namespace hcfp4;
 // Set when a bounded wait expired; part of the device image, so no call has to allocate it.
 __device__ uint32_t g_error;
 
-template <int BN, bool GLU>
+template <bool GLU>
 __global__ void __launch_bounds__(kGemmThreads, 1) Fp4GemmKernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape shape)
 {
-    GemmLoop<BN, GLU>(&maps, shape);
+    GemmLoop<GLU>(&maps, shape);
 }
 
 template <bool GLU>
@@ -36,7 +36,7 @@ template <typename Kernel> bool AllowShared(Kernel *kernel)
     cudaGetLastError();
     return false;
 }
-cudaLaunchConfig_t Config(cudaLaunchAttribute *at, int ctas, int clusterCtas, int smem, void *stream)
+cudaLaunchConfig_t LaunchConfig(cudaLaunchAttribute *at, int ctas, int clusterCtas, int smem, void *stream)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, 1, 1);
@@ -58,10 +58,9 @@ bool CurrentDevice(Device *d)
     bool good = true;
     *d = devices.Get(dev, [&](Device *v) {
         good = cudaDeviceGetAttribute(&v->sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && cudaGetSymbolAddress((void **)&v->error, g_error) == cudaSuccess &&
-               AllowShared(Fp4GemmKernel<128, false>) && AllowShared(Fp4GemmKernel<256, false>) && AllowShared(Fp4GemmKernel<256, true>) &&
-               AllowShared(Fp4GemmPairKernel<false>) && AllowShared(Fp4GemmPairKernel<true>);
+               AllowShared(Fp4GemmKernel<false>) && AllowShared(Fp4GemmKernel<true>) && AllowShared(Fp4GemmPairKernel<false>) && AllowShared(Fp4GemmPairKernel<true>);
         cudaLaunchAttribute at[2];
-        const cudaLaunchConfig_t cfg = Config(at, v->sms / 2 * 2, 2, PairSmemBytes(kMaxExperts), nullptr);
+        const cudaLaunchConfig_t cfg = LaunchConfig(at, v->sms / 2 * 2, 2, PairSmemBytes(kMaxExperts), nullptr);
         good = good && cudaOccupancyMaxActiveClusters(&v->pairs, Fp4GemmPairKernel<true>, &cfg) == cudaSuccess;
         if (!good) cudaGetLastError();
         return good;
@@ -89,7 +88,7 @@ HcclResult ScaleMap(CUtensorMap *m, const void *scales, int64_t tiles)
 template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clusterCtas, int smem, void *stream, const Maps &maps, const Shape &shape)
 {
     cudaLaunchAttribute at[2];
-    const cudaLaunchConfig_t cfg = Config(at, ctas, clusterCtas, smem, stream);
+    const cudaLaunchConfig_t cfg = LaunchConfig(at, ctas, clusterCtas, smem, stream);
     return cudaLaunchKernelEx(&cfg, kernel, maps, shape);
 }
 
@@ -125,8 +124,7 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     // Rows of A by the tile: all there may be, or as many as an expert has on average (how many it has is known on the device only).
     const int64_t pairTiles = experts > 0 ? (M + 255) / 256 + std::min(M, experts) / 2 : (M + 255) / 256;
     const bool pairs = dev.pairs > 0 && pairTiles * columns >= dev.pairs && (experts == 0 ? M > 128 : M >= 128 * experts);
-    const bool wideTile = pairs || glu || rowTiles * ((N + 127) / 128) >= 4 * dev.sms;
-    g.tilesN = wideTile ? (int)columns : (N + 127) / 128;
+    g.tilesN = pairs ? (int)columns : (N + 127) / 128;
     g.group = pairs ? 8 : 16;
     if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX || rowTiles * g.tileCols > INT32_MAX) {
         RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
@@ -140,6 +138,8 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
         while (g.boxRows > 8 && g.boxRows / 2 >= likely) g.boxRows /= 2;
         if (experts > 0) g.boxRows = likely >= 96 ? 128 : 32;
     }
+    g.aSlot = Config<128>::ASlot(g.boxRows, experts > 0);
+    g.stages = glu ? Config<256>::Stages(g.aSlot, experts) : Config<128>::Stages(g.aSlot, experts);
     Maps maps;
     CHK_RET(ValueMap(&maps.a, a.values, 1, M, K, g.boxRows));
     CHK_RET(ScaleMap(&maps.sa, a.scales, rowTiles * g.tileCols));
@@ -153,9 +153,10 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     if (pairs) {
         const int both = 2 * (int)std::min<int64_t>(dev.pairs, (experts > 0 ? rowTiles : pairTiles) * g.tilesN);
         e = glu ? Launch(Fp4GemmPairKernel<true>, both, 2, PairSmemBytes(experts), stream, maps, g) : Launch(Fp4GemmPairKernel<false>, both, 2, PairSmemBytes(experts), stream, maps, g);
-    } else if (glu) e = Launch(Fp4GemmKernel<256, true>, ctas, 1, SmemBytes<256>(experts), stream, maps, g);
-    else if (wideTile) e = Launch(Fp4GemmKernel<256, false>, ctas, 1, SmemBytes<256>(experts), stream, maps, g);
-    else e = Launch(Fp4GemmKernel<128, false>, ctas, 1, SmemBytes<128>(experts), stream, maps, g);
+    } else {
+        e = glu ? Launch(Fp4GemmKernel<true>, ctas, 1, Config<256>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g)
+                : Launch(Fp4GemmKernel<false>, ctas, 1, Config<128>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g);
+    }
     if (e != cudaSuccess) {
         cudaGetLastError();
         HCCL_ERROR("%s launch failed: %s", what, cudaGetErrorString(e));

@@ -1,24 +1,29 @@
-// fp4_gemm.cuh - persistent main loop of products of microscaled 4-bit operands (tcgen05 kind::mxf4, block scaling).
+// fp4_gemm.cuh - products of microscaled 4-bit operands (tcgen05 kind::mxf4, block scaling), and the loop for few rows.
 //
-//   D[m][n] = sum over blocks b of 32 columns of  2^(sa[m][b] + sb[n][b] - 254) * sum over the block of a[m][c] b[n][c]
+//   out[m][n] = sum over blocks b of 32 columns of  2^(sa[m][b] + sb[n][b] - 254) * sum over the block of a[m][c] b[n][c]
 //
 // The tensor core applies the scales: besides the operand tiles in shared memory (64 columns, 32 bytes a row and
 // instruction) it wants the scale bytes in tensor memory, where row r of an operand finds the four bytes of 128 columns in lane
 // r % 32, column r / 32 of each quarter - which is how the tiles of scales are laid out in memory, so that one 512-byte
 // copy (tcgen05.cp, 32 lanes x 16 bytes, repeated for the four quarters) per operand, 128 rows and 128 columns puts them there.
 //
+// In the loop of this file the operands change places: 128 rows of B, the weights, are the instruction's M, and up to 128 rows of A,
+// the tokens, its N, which is rounded up to 16 from what there is.  A product of 128 x 64 by 16 x 64 reads 4.5 KB of shared memory where
+// the other way round it would read 8 KB for 128 rows of which 16 are real (16 x 8192 by one tile of weights: BACK us, so FRONT).
+// Many rows go to the loop of fp4_gemm_pair.cuh.
+//
 // Warp roles:
-//   warp 0      TMA producer: 256 columns a stage - rows of A and B (128-byte swizzle) and their tiles of scales
+//   warp 0      TMA producer: 256 columns a stage - rows of both operands (128-byte swizzle) and their tiles of scales
 //   warp 1      issuer: copies a stage's scales to tensor memory, then four products of 64 columns; one thread
 //   warps 4-11  epilogue: first the whole accumulator as bf16 into registers, which hands it back to the issuer after a few hundred
-//               cycles, then through shared memory out in whole segments of the result's rows
+//               cycles, then out
 // Each stage of the ring has its own columns for scales in tensor memory, so that the barrier that frees the stage frees them too.
 //
-// Rows of A may be grouped by expert, with a matrix of B for each: tiles never cross a group; what a tile loads behind its
-// group's last row are other rows' values, which no stored row depends on.
+// Rows of A may be grouped by expert, with a matrix of B for each: tiles never cross a group; what a tile holds behind its
+// group's last row are other rows' values, which no stored value depends on.
 //
-// A gated product (GLU) loads 128 rows of each of two matrices instead of 256 of one; its epilogue has gate and up of the same
-// column in one thread and stores silu(gate) * up.
+// A gated product (GLU) loads 128 rows of each of two matrices and keeps two accumulators, gate and up of the same element in the
+// same lane and thread, and stores silu(gate) * up.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -32,8 +37,6 @@ constexpr int kStageCols = 256;             // columns of K a stage, 128 bytes
 constexpr int kUmmaCols = 64;               // of an instruction
 constexpr int kStoreWarps = 8;                        // of the epilogue: two for each quarter of the accumulator's rows
 constexpr int kGemmThreads = 32 * (4 + kStoreWarps);
-constexpr int kSlabCols = 32;               // columns that an epilogue warp stages at a time
-constexpr int kSlabBytes = 32 * kSlabCols * 2;
 
 struct Maps { CUtensorMap a, sa, b[2], sb[2]; };        // b[1], sb[1]: the second matrix of a gated product, else the first again
 
@@ -42,6 +45,7 @@ struct Shape {
     int tilesN;
     int group;                  // row tiles that are taken together before the next column of tiles
     int boxRows;                // rows of A that a load takes: a tile loads no more than it needs (one CTA a tile)
+    int aSlot, stages;          // bytes of A in a stage; stages of the ring
     int experts;                // 0: one matrix
     const int32_t *offsets;
     int tileCols, tileRowsB;    // tiles of scales along K; along N of one matrix
@@ -50,28 +54,34 @@ struct Shape {
     uint32_t *error;
 };
 
-template <int BN> struct Config {
-    static_assert(BN == 128 || BN == 256, "one or two tiles of scales wide");
-    static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
-    static constexpr int kSaBytes = 2 * kTileBytes, kSbBytes = BN / 128 * 2 * kTileBytes;
-    static constexpr int kStageBytes = kABytes + kBBytes + kSaBytes + kSbBytes;
-    static constexpr int kStages = BN == 256 ? 4 : 6;
-    static constexpr int kAccumulators = BN == 256 ? 1 : 2;
-    static constexpr int kScaleCols = 8 + BN / 128 * 8;             // of a stage, in tensor memory
-    static constexpr int kScaleBase = kAccumulators * BN;
-    static_assert(kScaleBase + kStages * kScaleCols <= 512, "tensor memory");
-};
-
+constexpr int kMaxStages = 12;
 struct State {
-    uint64_t full[8], empty[8], accFull[2], accEmpty[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], accFull[2], accEmpty[2];
     uint32_t tmem;
     volatile uint32_t abort;
 };
-// Behind the ring: the epilogue's slabs, the barriers, and with grouped rows where they start.
-template <int BN> constexpr int SmemBytes(int experts)
-{
-    return 1024 + Config<BN>::kStages * Config<BN>::kStageBytes + kStoreWarps * kSlabBytes + 256 + (experts > 0 ? 4 * (experts + 1) : 0);
-}
+static_assert(sizeof(State) <= 256, "barriers");
+
+// A CTA's shared memory: the stages' rows of A, then those of B, their tiles of scales, the barriers, and with
+// grouped rows where they start.  A stage of A is as large as a load of it, so that few rows leave room for more stages: one
+// product after the other takes as long as a load is under way divided by the stages (16 x 28672 x 8192 with six of them SIX us, with ten TEN).  The
+// tensor core reads 128 rows all the same, those behind from whatever lies there: rows of B at the worst, never behind the allocation.
+template <int BN> struct Config {
+    static_assert(BN == 128 || BN == 256, "one or two tiles of scales wide");
+    static constexpr int kBBytes = BN * 128, kSaBytes = 2 * kTileBytes, kSbBytes = BN / 128 * 2 * kTileBytes;
+    static constexpr int kAccumulators = BN == 256 ? 1 : 2;
+    static constexpr int kScaleCols = 8 + BN / 128 * 8;             // of a stage, in tensor memory
+    static constexpr int kScaleBase = kAccumulators * BN;
+    static constexpr int kTail = 256;
+    __host__ __device__ static constexpr int ASlot(int boxRows, bool grouped) { return grouped || boxRows > 64 ? 128 * 128 : boxRows < 8 ? 1024 : boxRows * 128; }
+    static constexpr int StageBytes(int aSlot) { return aSlot + kBBytes + kSaBytes + kSbBytes; }
+    static constexpr int Stages(int aSlot, int experts)
+    {
+        const int room = 227 * 1024 - 1024 - kTail - (experts > 0 ? 4 * (experts + 1) : 0), fit = room / StageBytes(aSlot), columns = (512 - kScaleBase) / kScaleCols;
+        return fit < columns ? (fit < kMaxStages ? fit : kMaxStages) : (columns < kMaxStages ? columns : kMaxStages);
+    }
+    static constexpr int SmemBytes(int aSlot, int stages, int experts) { return 1024 + stages * StageBytes(aSlot) + kTail + (experts > 0 ? 4 * (experts + 1) : 0); }
+};
 
 // kind::mxf4: e2m1 x e2m1 with scales that are powers of two, both operands with K contiguous.  The fields of the scales' byte
 // pairs (bits 4-5 for B, 29-30 for A) are set for each instruction: 0 for the first 64 of 128 columns, 2 for the others.
@@ -79,22 +89,28 @@ __host__ __device__ constexpr uint32_t InstrDescMxf4(uint32_t M, uint32_t N, uin
 {
     return (pair << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24) | (pair << 29);
 }
-// 32 rows of 16 bytes, no swizzle: groups of eight rows 128 bytes apart.
-__device__ __forceinline__ uint64_t ScaleDesc(const void *tile)
-{
-    return (uint64_t)((SmemAddr(tile) & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
-}
-__device__ __forceinline__ void CopyScales(uint32_t tmem, uint64_t desc)
-{
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void MmaMxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool accumulate)
+// Descriptors of shared memory in two words, so that the issuing thread steps through a ring with 32-bit additions: it has a few
+// hundred cycles a stage for eight and more instructions and their operands (with descriptors made anew for each: PLAIN us
+// for 16 x 28672 x 8192, so LOW).  The low word has the address in units of 16 bytes; the high ones say: K contiguous, rows of 128 bytes with
+// the 128-byte swizzle, 1024 bytes from eight rows to the next eight; and 32 rows of 16 bytes of scales, eight rows in 128 bytes.
+constexpr uint32_t kRowsHigh = (1024 >> 4) | (1u << 14) | (2u << 29), kScalesHigh = (128 >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t DescLow(const void *p) { return ((SmemAddr(p) & 0x3FFFF) >> 4) | (1u << 16); }
+__device__ __forceinline__ void CopyScales(uint32_t tmem, uint32_t low)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .b64 d;\n\t"
+        "mov.b64 d, {%1, %2};\n\t"
+        "tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem), "r"(low), "r"(kScalesHigh) : "memory");
+}
+__device__ __forceinline__ void MmaMxf4(uint32_t d, uint32_t aLow, uint32_t bLow, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate ? 1u : 0u) : "memory");
+        "mov.b64 a, {%1, %7};\n\t"
+        "mov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "r"(aLow), "r"(bLow), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(kRowsHigh) : "memory");
 }
 __device__ __forceinline__ void TmaLoad3d(void *dst, const CUtensorMap *m, uint64_t *bar, int32_t x, int32_t y, int32_t z)
 {
@@ -149,86 +165,74 @@ __device__ __forceinline__ uint32_t Bf16Pair(float a, float b)
 // value.  An exact one calls a subroutine where a lane's operand is out of the ordinary: 60 us a tile, measured.
 __device__ __forceinline__ float SiluTimes(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-// 32 rows x 32 columns of a warp leave through its slab: four lanes write a row's 64 bytes.  Pieces of 16 bytes are exchanged by
-// the row so that neither side meets bank conflicts beyond those of the width.
-__device__ __forceinline__ void StoreSlab(uint8_t *slab, const uint32_t (&packed)[16], int lane, int rows, __nv_bfloat16 *out, int64_t ld, int cols, bool wide)
+// A warp's part of a finished accumulator, the operands in each other's places: lane l has row 32 q + l of the weights, columns are
+// tokens, 64 of them the warp's.  handBack is called once they are in registers; two lanes exchange every other value, so that each
+// stores two neighbours.
+template <bool GLU, typename HandBack>
+__device__ __forceinline__ void StoreTokens(const Shape &g, const Tile &t, uint32_t accumulator, int warp, int lane, bool pairs, HandBack handBack)
 {
+    const int q = warp & 3, first = (warp >> 2) * 64, tokens = t.rows - first, n = t.column * 128 + q * 32 + lane;
+    uint32_t packed[32];            // two tokens each
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-        *(uint4 *)(slab + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) = make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
-    __syncwarp();
-    const int piece = lane & 3;
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-        const int row = it * 8 + (lane >> 2);
-        if (row >= rows) continue;
-        const uint4 v = *(const uint4 *)(slab + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
-        __nv_bfloat16 *at = out + (int64_t)row * ld + piece * 8;
-        if (wide && piece * 8 + 8 <= cols) *(uint4 *)at = v;
-        else
-            for (int i = 0; i < 8 && piece * 8 + i < cols; ++i) at[i] = ((const __nv_bfloat16 *)&v)[i];
-    }
-    __syncwarp();
-}
-
-// A warp's 32 rows and half of the columns of a finished accumulator.  handBack is called once they are in registers: the next
-// tile's products start while these are on their way out (8192 x 28672 x 8192 by pairs of CTAs: BEFORE us with it at the end, AFTER so).
-template <int BN, bool GLU, typename HandBack>
-__device__ __forceinline__ void StoreTile(const Shape &g, const Tile &t, uint32_t accumulator, int warp, int lane, uint8_t *slab, bool wide, HandBack handBack)
-{
-    constexpr int kOut = GLU ? BN / 2 : BN, kMine = kOut / 2, kSlabs = kMine / kSlabCols;
-    const int q = warp & 3, first = (warp >> 2) * kMine;
-    const int rows = t.rows - q * 32, cols = g.N - t.column * kOut - first;
-    uint32_t packed[kSlabs][16];
-    if (rows > 0) {
-        const uint32_t from = accumulator + ((uint32_t)(q * 32) << 16) + first;
-#pragma unroll
-        for (int c = 0; c < kSlabs; ++c) {
+    for (int c = 0; c < 64; c += 32) {
+        if (tokens > c) {
             uint32_t v[32];
-            TmemLoad32x32(from + c * kSlabCols, v);
+            const uint32_t from = accumulator + ((uint32_t)(q * 32) << 16) + first + c;
+            TmemLoad32x32(from, v);
             if constexpr (GLU) {
                 uint32_t u[32];
-                TmemLoad32x32(from + kOut + c * kSlabCols, u);
+                TmemLoad32x32(from + 128, u);
                 TmemLoadWait();
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    packed[c][j] = Bf16Pair(SiluTimes(__uint_as_float(v[2 * j]), __uint_as_float(u[2 * j])), SiluTimes(__uint_as_float(v[2 * j + 1]), __uint_as_float(u[2 * j + 1])));
+                    packed[c / 2 + j] = Bf16Pair(SiluTimes(__uint_as_float(v[2 * j]), __uint_as_float(u[2 * j])), SiluTimes(__uint_as_float(v[2 * j + 1]), __uint_as_float(u[2 * j + 1])));
             } else {
                 TmemLoadWait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) packed[c][j] = Bf16Pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                for (int j = 0; j < 16; ++j) packed[c / 2 + j] = Bf16Pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
             }
         }
     }
     TcFenceBefore();
     __syncwarp();
     if (lane == 0) handBack();
-    if (rows > 0) {
-        __nv_bfloat16 *out = g.out + (int64_t)(t.row + q * 32) * g.ldOut + t.column * kOut + first;
+    __nv_bfloat16 *out = g.out + (int64_t)(t.row + first) * g.ldOut;
 #pragma unroll
-        for (int c = 0; c < kSlabs; ++c)
-            if (c * kSlabCols < cols) StoreSlab(slab, packed[c], lane, rows, out + c * kSlabCols, g.ldOut, cols - c * kSlabCols, wide);
+    for (int j = 0; j < 32; ++j) {
+        if (2 * j >= tokens) break;
+        if (pairs) {
+            // the even lane stores token 2 j for both, the odd one token 2 j + 1
+            const uint32_t mine = packed[j], other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            const int token = 2 * j + (lane & 1);
+            const uint32_t both = lane & 1 ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+            __nv_bfloat16 *at = out + (int64_t)token * g.ldOut + (n & ~1);
+            if (token < tokens) {
+                if ((n | 1) < g.N) *(uint32_t *)at = both;
+                else if ((n & ~1) < g.N) *at = *(const __nv_bfloat16 *)&both;
+            }
+        } else if (n < g.N) {
+            const __nv_bfloat162 both = *(const __nv_bfloat162 *)&packed[j];
+            out[(int64_t)(2 * j) * g.ldOut + n] = both.x;
+            if (2 * j + 1 < tokens) out[(int64_t)(2 * j + 1) * g.ldOut + n] = both.y;
+        }
     }
 }
 
-static_assert(SmemBytes<128>(kMaxExperts) <= 227 * 1024 && SmemBytes<256>(kMaxExperts) <= 227 * 1024, "shared memory");
-
-template <int BN, bool GLU>
-__device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
+template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
 {
+    constexpr int BN = GLU ? 256 : 128;         // rows of weights: gate and up take 128 each
     using Cfg = Config<BN>;
-    static_assert(!GLU || BN == 256, "gate and up take 128 rows each");
     extern __shared__ uint8_t smemRaw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);
-    uint8_t *slabs = smem + Cfg::kStages * Cfg::kStageBytes;
-    State *st = (State *)(slabs + kStoreWarps * kSlabBytes);
-    static_assert(sizeof(State) <= 256, "barriers");
+    const int ring = g.stages;
+    uint8_t *const ringB = smem + ring * g.aSlot, *const ringSa = ringB + ring * Cfg::kBBytes, *const ringSb = ringSa + ring * Cfg::kSaBytes;
+    State *st = (State *)(ringSb + ring * Cfg::kSbBytes);
     int *start = (int *)((uint8_t *)st + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int stages = (g.K + kStageCols - 1) / kStageCols;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Cfg::kStages; ++s) { MbarInit(&st->full[s], 1); MbarInit(&st->empty[s], 1); }
+        for (int s = 0; s < ring; ++s) { MbarInit(&st->full[s], 1); MbarInit(&st->empty[s], 1); }
         for (int a = 0; a < 2; ++a) { MbarInit(&st->accFull[a], 1); MbarInit(&st->accEmpty[a], kStoreWarps); }
         st->abort = 0;
         MbarFenceInit();
@@ -252,27 +256,27 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
         // ------------------------------------------------------------------------------- TMA producer
         if (ElectOne()) {
             GridDependencyWait();
-            uint32_t it = 0;
+            int s = 0;
+            uint32_t phase = 0;         // of the ring: flips each time round
             bool alive = true;
             Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
-                const int n = t.column * (GLU ? 128 : BN);
-                const int boxes = (t.rows + g.boxRows - 1) / g.boxRows, bytes = Cfg::kStageBytes - Cfg::kABytes + boxes * g.boxRows * 128;
-                for (int k = 0; k < stages; ++k, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!MbarWait(&st->empty[s], ((it / Cfg::kStages) & 1) ^ 1, &st->abort)) { alive = false; break; }
-                    uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
+                const int n = t.column * 128;
+                const int boxes = (t.rows + g.boxRows - 1) / g.boxRows, bytes = Cfg::StageBytes(boxes * g.boxRows * 128);
+                for (int k = 0; k < stages; ++k) {
+                    if (!MbarWait(&st->empty[s], phase ^ 1, &st->abort)) { alive = false; break; }
+                    uint8_t *a = smem + s * g.aSlot, *b = ringB + s * Cfg::kBBytes, *sa = ringSa + s * Cfg::kSaBytes, *sb = ringSb + s * Cfg::kSbBytes;
                     MbarExpectTx(&st->full[s], bytes);
                     // as many coordinates as the map has dimensions; rows that are not loaded hold what was there, and are not stored
                     for (int r = 0; r < boxes; ++r) TmaLoad3d(a + r * g.boxRows * 128, &maps->a, &st->full[s], k * 128, t.row + r * g.boxRows, 0);
                     TmaLoad2d(sa, &maps->sa, &st->full[s], 0, t.scaleTile * g.tileCols + 2 * k);
 #pragma unroll
                     for (int h = 0; h < BN / 128; ++h) {
-                        const int which = GLU ? h : 0, row = GLU ? n : n + h * 128;
-                        TmaLoad3d(b + h * 16384, &maps->b[which], &st->full[s], k * 128, row, t.expert);
-                        TmaLoad2d(sb + h * 2 * kTileBytes, &maps->sb[which], &st->full[s], 0, (t.expert * g.tileRowsB + row / 128) * g.tileCols + 2 * k);
+                        TmaLoad3d(b + h * 16384, &maps->b[h], &st->full[s], k * 128, n, t.expert);
+                        TmaLoad2d(sb + h * 2 * kTileBytes, &maps->sb[h], &st->full[s], 0, (t.expert * g.tileRowsB + t.column) * g.tileCols + 2 * k);
                     }
+                    if (++s == ring) { s = 0; phase ^= 1; }
                 }
             }
             if (!alive) __nanosleep(500000);        // copies under way still write here: they end long before this does
@@ -281,38 +285,44 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
         // -------------------------------------------------------------------------------------- issuer
         if (ElectOne()) {
             GridDependencyWait();
-            uint32_t it = 0, i = 0;
+            int s = 0;
+            uint32_t phase = 0, i = 0;
+            const uint32_t lowA = DescLow(smem), lowB = DescLow(ringB), lowSa = DescLow(ringSa), lowSb = DescLow(ringSb);
             bool alive = true;
             Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
-                const uint32_t acc = i % Cfg::kAccumulators, phase = (i / Cfg::kAccumulators) & 1;
+                const uint32_t acc = i % Cfg::kAccumulators, accPhase = (i / Cfg::kAccumulators) & 1;
                 ++i;
-                if (!MbarWait(&st->accEmpty[acc], phase ^ 1, &st->abort)) { alive = false; break; }
+                if (!MbarWait(&st->accEmpty[acc], accPhase ^ 1, &st->abort)) { alive = false; break; }
                 TcFenceAfter();
-                const uint32_t d = tmem + acc * BN;
-                for (int k = 0; k < stages; ++k, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!MbarWait(&st->full[s], (it / Cfg::kStages) & 1, &st->abort)) { alive = false; break; }
+                const uint32_t d = tmem + acc * BN, tokens = (uint32_t)(t.rows + 15) / 16 * 16;
+                const uint32_t idesc[2] = {InstrDescMxf4(128, tokens, 0), InstrDescMxf4(128, tokens, 2)};
+                uint32_t more = 0;
+                for (int k = 0; k < stages; ++k) {
+                    if (!MbarWait(&st->full[s], phase, &st->abort)) { alive = false; break; }
                     TcFenceAfter();
-                    uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
+                    const uint32_t a = lowA + s * (g.aSlot >> 4), b = lowB + s * (Cfg::kBBytes >> 4), sa = lowSa + s * (Cfg::kSaBytes >> 4), sb = lowSb + s * (Cfg::kSbBytes >> 4);
                     const uint32_t ta = tmem + Cfg::kScaleBase + s * Cfg::kScaleCols, tb = ta + 8;
                     const int left = g.K - k * kStageCols;
                     // scales of A: columns 0-3 the first 128 of K, 4-7 the second; of B likewise, with four more for each 128 rows
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         if (c * kTileCols >= left) break;
-                        CopyScales(ta + c * 4, ScaleDesc(sa + c * kTileBytes));
+                        CopyScales(ta + c * 4, sa + c * (kTileBytes >> 4));
 #pragma unroll
-                        for (int h = 0; h < BN / 128; ++h) CopyScales(tb + c * (BN / 32) + h * 4, ScaleDesc(sb + (h * 2 + c) * kTileBytes));
+                        for (int h = 0; h < BN / 128; ++h) CopyScales(tb + c * (BN / 32) + h * 4, sb + (h * 2 + c) * (kTileBytes >> 4));
                     }
-                    const uint64_t da = SmemDescKMajorSw128(a), db = SmemDescKMajorSw128(b);
 #pragma unroll
                     for (int u = 0; u < kStageCols / kUmmaCols; ++u) {
                         if (u * kUmmaCols >= left) break;
-                        MmaMxf4(d, da + u * 2, db + u * 2, InstrDescMxf4(128, BN, (u & 1) * 2), ta + (u >> 1) * 4, tb + (u >> 1) * (BN / 32), (k | u) != 0);
+#pragma unroll
+                        for (int h = 0; h < BN / 128; ++h)
+                            MmaMxf4(d + h * 128, b + h * (16384 >> 4) + u * 2, a + u * 2, idesc[u & 1], tb + (u >> 1) * (BN / 32) + h * 4, ta + (u >> 1) * 4, more);
+                        more = 1;
                     }
                     MmaCommit(&st->empty[s]);
+                    if (++s == ring) { s = 0; phase ^= 1; }
                 }
                 if (alive) MmaCommit(&st->accFull[acc]);
             }
@@ -320,8 +330,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
     } else if (warp >= 4) {
         // ------------------------------------------------------------------------------------ epilogue
         GridDependencyWait();
-        uint8_t *slab = slabs + (warp - 4) * kSlabBytes;
-        const bool wide = g.ldOut % 8 == 0 && ((uintptr_t)g.out & 15) == 0;
+        const bool pairs = g.ldOut % 2 == 0 && ((uintptr_t)g.out & 3) == 0;
         uint32_t i = 0;
         Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
         Tile t;
@@ -331,7 +340,7 @@ __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
             if (!MbarWait(&st->accFull[acc], phase, &st->abort)) break;
             __syncwarp();
             TcFenceAfter();
-            StoreTile<BN, GLU>(g, t, tmem + acc * BN, warp - 4, lane, slab, wide, [&] { MbarArrive(&st->accEmpty[acc]); });
+            StoreTokens<GLU>(g, t, tmem + acc * BN, warp - 4, lane, pairs, [&] { MbarArrive(&st->accEmpty[acc]); });
         }
     }
     // ---------------------------------------------------------------------------------------- the end

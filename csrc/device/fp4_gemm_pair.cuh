@@ -14,6 +14,9 @@
 
 namespace hcfp4 {
 
+constexpr int kSlabCols = 32;               // columns that an epilogue warp stages at a time
+constexpr int kSlabBytes = 32 * kSlabCols * 2;
+
 template <int STAGES> struct PairConfig {
     static constexpr int kStages = STAGES;
     static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128, kSaBytes = 2 * kTileBytes, kSbBytes = 2 * 2 * kTileBytes;
@@ -27,22 +30,89 @@ constexpr int PairSmemBytes(int experts)
     return 1024 + kPairStages * PairConfig<kPairStages>::kStageBytes + kStoreWarps * kSlabBytes + 256 + (experts > 0 ? 4 * (experts + 1) : 0);
 }
 
-__device__ __forceinline__ void CopyScalesPair(uint32_t tmem, uint64_t desc)
-{
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void MmaMxf4Pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool accumulate)
+__device__ __forceinline__ void CopyScalesPair(uint32_t tmem, uint32_t low)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .b64 d;\n\t"
+        "mov.b64 d, {%1, %2};\n\t"
+        "tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(tmem), "r"(low), "r"(kScalesHigh) : "memory");
+}
+__device__ __forceinline__ void MmaMxf4Pair(uint32_t d, uint32_t aLow, uint32_t bLow, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate ? 1u : 0u) : "memory");
+        "mov.b64 a, {%1, %7};\n\t"
+        "mov.b64 b, {%2, %7};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "r"(aLow), "r"(bLow), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(kRowsHigh) : "memory");
 }
 __device__ __forceinline__ void TmaLoad3dPair(void *dst, const CUtensorMap *m, uint32_t bar, int32_t x, int32_t y, int32_t z)
 {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(SmemAddr(dst)), "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// 32 rows x 32 columns of a warp leave through its slab: four lanes write a row's 64 bytes.  Pieces of 16 bytes are exchanged by
+// the row so that neither side meets bank conflicts beyond those of the width.
+__device__ __forceinline__ void StoreSlab(uint8_t *slab, const uint32_t (&packed)[16], int lane, int rows, __nv_bfloat16 *out, int64_t ld, int cols, bool wide)
+{
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+        *(uint4 *)(slab + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)) = make_uint4(packed[4 * v], packed[4 * v + 1], packed[4 * v + 2], packed[4 * v + 3]);
+    __syncwarp();
+    const int piece = lane & 3;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int row = it * 8 + (lane >> 2);
+        if (row >= rows) continue;
+        const uint4 v = *(const uint4 *)(slab + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+        __nv_bfloat16 *at = out + (int64_t)row * ld + piece * 8;
+        if (wide && piece * 8 + 8 <= cols) *(uint4 *)at = v;
+        else
+            for (int i = 0; i < 8 && piece * 8 + i < cols; ++i) at[i] = ((const __nv_bfloat16 *)&v)[i];
+    }
+    __syncwarp();
+}
+
+// A warp's 32 rows and half of the columns of a finished accumulator.  handBack is called once they are in registers: the next
+// tile's products start while these are on their way out (8192 x 28672 x 8192: 718 us by four warps and with it at the end, 663 so).
+template <bool GLU, typename HandBack>
+__device__ __forceinline__ void StoreTile(const Shape &g, const Tile &t, uint32_t accumulator, int warp, int lane, uint8_t *slab, bool wide, HandBack handBack)
+{
+    constexpr int kOut = GLU ? 128 : 256, kMine = kOut / 2, kSlabs = kMine / kSlabCols;
+    const int q = warp & 3, first = (warp >> 2) * kMine;
+    const int rows = t.rows - q * 32, cols = g.N - t.column * kOut - first;
+    uint32_t packed[kSlabs][16];
+    if (rows > 0) {
+        const uint32_t from = accumulator + ((uint32_t)(q * 32) << 16) + first;
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c) {
+            uint32_t v[32];
+            TmemLoad32x32(from + c * kSlabCols, v);
+            if constexpr (GLU) {
+                uint32_t u[32];
+                TmemLoad32x32(from + kOut + c * kSlabCols, u);
+                TmemLoadWait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    packed[c][j] = Bf16Pair(SiluTimes(__uint_as_float(v[2 * j]), __uint_as_float(u[2 * j])), SiluTimes(__uint_as_float(v[2 * j + 1]), __uint_as_float(u[2 * j + 1])));
+            } else {
+                TmemLoadWait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) packed[c][j] = Bf16Pair(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            }
+        }
+    }
+    TcFenceBefore();
+    __syncwarp();
+    if (lane == 0) handBack();
+    if (rows > 0) {
+        __nv_bfloat16 *out = g.out + (int64_t)(t.row + q * 32) * g.ldOut + t.column * kOut + first;
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+            if (c * kSlabCols < cols) StoreSlab(slab, packed[c], lane, rows, out + c * kSlabCols, g.ldOut, cols - c * kSlabCols, wide);
+    }
 }
 
 template <bool GLU> __device__ __forceinline__ void GemmLoopPair(const Maps *maps, const Shape &g)
@@ -113,7 +183,9 @@ template <bool GLU> __device__ __forceinline__ void GemmLoopPair(const Maps *map
         // -------------------------------------------------------------------- issuer (leader CTA only)
         if (leader && ElectOne()) {
             GridDependencyWait();
-            uint32_t it = 0, i = 0;
+            int s = 0;
+            uint32_t phase = 0, i = 0;
+            const uint32_t low = DescLow(smem);
             bool alive = true;
             Tiles<256> tiles(g, start, first, step, rank);
             Tile t;
@@ -121,27 +193,28 @@ template <bool GLU> __device__ __forceinline__ void GemmLoopPair(const Maps *map
                 if (!MbarWait(&st->accEmpty[0], (i & 1) ^ 1, &st->abort)) { alive = false; break; }
                 ++i;
                 TcFenceAfter();
-                for (int k = 0; k < stages; ++k, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!MbarWait(&st->full[s], (it / Cfg::kStages) & 1, &st->abort)) { alive = false; break; }
+                uint32_t more = 0;
+                for (int k = 0; k < stages; ++k) {
+                    if (!MbarWait(&st->full[s], phase, &st->abort)) { alive = false; break; }
                     TcFenceAfter();
-                    uint8_t *a = smem + s * Cfg::kStageBytes, *b = a + Cfg::kABytes, *sa = b + Cfg::kBBytes, *sb = sa + Cfg::kSaBytes;
+                    const uint32_t a = low + s * (Cfg::kStageBytes >> 4), b = a + (Cfg::kABytes >> 4), sa = b + (Cfg::kBBytes >> 4), sb = sa + (Cfg::kSaBytes >> 4);
                     const uint32_t ta = tmem + Cfg::kScaleBase + s * Cfg::kScaleCols, tb = ta + 8;
                     const int left = g.K - k * kStageCols;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         if (c * kTileCols >= left) break;
-                        CopyScalesPair(ta + c * 4, ScaleDesc(sa + c * kTileBytes));
+                        CopyScalesPair(ta + c * 4, sa + c * (kTileBytes >> 4));
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) CopyScalesPair(tb + c * 8 + h * 4, ScaleDesc(sb + (h * 2 + c) * kTileBytes));
+                        for (int h = 0; h < 2; ++h) CopyScalesPair(tb + c * 8 + h * 4, sb + (h * 2 + c) * (kTileBytes >> 4));
                     }
-                    const uint64_t da = SmemDescKMajorSw128(a), db = SmemDescKMajorSw128(b);
 #pragma unroll
                     for (int u = 0; u < kStageCols / kUmmaCols; ++u) {
                         if (u * kUmmaCols >= left) break;
-                        MmaMxf4Pair(tmem, da + u * 2, db + u * 2, InstrDescMxf4(256, 256, (u & 1) * 2), ta + (u >> 1) * 4, tb + (u >> 1) * 8, (k | u) != 0);
+                        MmaMxf4Pair(tmem, a + u * 2, b + u * 2, InstrDescMxf4(256, 256, (u & 1) * 2), ta + (u >> 1) * 4, tb + (u >> 1) * 8, more);
+                        more = 1;
                     }
                     MmaCommitPair(&st->empty[s]);
+                    if (++s == Cfg::kStages) { s = 0; phase ^= 1; }
                 }
                 if (alive) MmaCommitPair(&st->accFull[0]);
             }
@@ -159,7 +232,7 @@ template <bool GLU> __device__ __forceinline__ void GemmLoopPair(const Maps *map
             ++i;
             __syncwarp();
             TcFenceAfter();
-            StoreTile<256, GLU>(g, t, tmem, warp - 4, lane, slab, wide, [&] {
+            StoreTile<GLU>(g, t, tmem, warp - 4, lane, slab, wide, [&] {
                 if (leader) MbarArrive(&st->accEmpty[0]);
                 else RemoteArrive(MapToCta(&st->accEmpty[0], 0));
             });

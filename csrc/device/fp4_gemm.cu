@@ -2,7 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <mutex>
+#include <cmath>
 
 #include "../../include/hcomm_fp4.h"
 #include "../core/log.h"
@@ -92,6 +92,32 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
     return cudaLaunchKernelEx(&cfg, kernel, maps, shape);
 }
 
+// Whether a product goes by pairs of CTAs (tiles of 256 rows x 256 columns, or 128 of a gated product) or by single CTAs (up to 128 rows x
+// 128 columns): the less of two estimates, in us.
+//   * tiles come in waves of what fits at once; of grouped rows, which are known on the device only, every expert is taken to have the
+//     average, and a tile that it fills half;
+//   * single: a stage of 256 columns of K takes 0.19 us to issue, or its bytes at 112 a ns; a tile at least 0.4 us and 2.8 a 128 rows, in which
+//     the tile in front is stored;
+//   * pair: 0.34 us a stage, and 1.5 in which nothing overlaps the reading of the tile's accumulator;
+//   * nothing is faster than its bytes at 6.5 TB/s.
+// us, single / pair: 500 x 3584 x 8192 13.7 / 15.1, 777 x 3584 x 8192 21.5 / 16.0, 256 x 8192 x 28672 34.8 / 41.1, 1024 x 1024 x 4096 9.0 / 10.0,
+// 2048 x 4096 x 1024 15.6 / 10.4, 4096 x 4096 x 4096 37.5 / 29.1, 8192 x 28672 x 8192 880 / 646; 32 experts, 7168 and 2048, gated and down: 64 rows
+// 66 / 81 and 37 / 53, 3000 95 / 112 and 60 / 67, 8000 142 / 140 and 107 / 89, 16000 237 / 225 and 180 / 144.
+struct Costs { double single, pair; };
+Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, int pairs)
+{
+    const double stages = (double)((K + kStageCols - 1) / kStageCols), matrices = experts > 0 ? std::min<double>((double)M, experts) : 1, rows = M / matrices;
+    auto tiles = [&](double tall, double wide) {
+        const double down = experts > 0 ? std::max(1.0, rows / tall + 0.5) : std::ceil(rows / tall);
+        return matrices * down * std::ceil(N / wide);
+    };
+    const double hbm = (17.0 / 32 * (M * K + matrices * (glu ? 2 : 1) * N * K) + 2.0 * M * N) / 6.5e6;
+    const double used = std::min(rows, 128.0), stage = std::max(0.19, ((glu ? 2 : 1) * 17408 + 1024 + 128 * used) / 112e3);
+    const double single = std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 2.8 * used / 128);
+    const double pair = std::ceil(tiles(256, glu ? 128 : 256) / std::max(pairs, 1)) * (stages * 0.34 + 1.5);
+    return {3.0 + std::max(single, hbm), 3.0 + std::max(pair, hbm)};
+}
+
 // b[1] is the up projection of a gated product, else NULL.
 HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, void *out, int M, int N, int K, int64_t ldOut, const int32_t *offsets, int experts, void *stream)
 {
@@ -120,18 +146,16 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     g.error = dev.error;
     const int matrices = std::max(experts, 1);
     const int64_t rowTiles = experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128;
-    const int64_t columns = glu ? (N + 127) / 128 : (N + 255) / 256;
-    // Rows of A by the tile: all there may be, or as many as an expert has on average (how many it has is known on the device only).
-    const int64_t pairTiles = experts > 0 ? (M + 255) / 256 + std::min(M, experts) / 2 : (M + 255) / 256;
-    const bool pairs = dev.pairs > 0 && pairTiles * columns >= dev.pairs && (experts == 0 ? M > 128 : M >= 128 * experts);
-    g.tilesN = pairs ? (int)columns : (N + 127) / 128;
+    const Costs costs = Estimate(M, N, K, experts, glu, dev.sms, dev.pairs);
+    const bool pairs = dev.pairs > 0 && M > 128 && costs.pair < costs.single;
+    g.tilesN = pairs && !glu ? (N + 255) / 256 : (N + 127) / 128;
     g.group = pairs ? 8 : 16;
     if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX || rowTiles * g.tileCols > INT32_MAX) {
         RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
         return HCCL_E_PARA;
     }
     // A SM's loads take some 55 bytes a cycle, rows outside the matrix as long as others: 16 x 18944 x 8192 with boxes of 128 rows
-    // BOX128 us, of 16 BOX16.  Rows of an expert, which are known on the device only, come in boxes of 32 where there are few of them.
+    // 20.6 us, of 16 16.4.  Rows of an expert, which are known on the device only, come in boxes of 32 where there are few of them.
     g.boxRows = 128;
     if (!pairs) {
         const int likely = experts > 0 ? M / experts : M;
@@ -151,7 +175,7 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     const int ctas = (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);
     cudaError_t e;
     if (pairs) {
-        const int both = 2 * (int)std::min<int64_t>(dev.pairs, (experts > 0 ? rowTiles : pairTiles) * g.tilesN);
+        const int both = 2 * (int)std::min<int64_t>(dev.pairs, rowTiles * g.tilesN);
         e = glu ? Launch(Fp4GemmPairKernel<true>, both, 2, PairSmemBytes(experts), stream, maps, g) : Launch(Fp4GemmPairKernel<false>, both, 2, PairSmemBytes(experts), stream, maps, g);
     } else {
         e = glu ? Launch(Fp4GemmKernel<true>, ctas, 1, Config<256>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g)
@@ -184,4 +208,10 @@ extern "C" int HcommFp4TakeError(void)
     if (cudaMemcpyFromSymbol(&v, g_error, sizeof(v)) != cudaSuccess) { cudaGetLastError(); return -1; }
     if (v) cudaMemcpyToSymbol(g_error, &zero, sizeof(zero));
     return (int)v;
+}
+// What the rule makes of a product on a device of that many SMs and pairs of CTAs at once: us by single CTAs and by pairs.
+extern "C" void HcommToolFp4Estimate(int M, int N, int K, int experts, int gated, int sms, int pairs, double *us)
+{
+    const Costs c = Estimate(M, N, K, experts, gated != 0, sms, pairs);
+    us[0] = c.single; us[1] = c.pair;
 }

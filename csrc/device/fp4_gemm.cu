@@ -29,7 +29,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) Fp4GemmPairKernel(const __gri
     GemmLoopPair<GLU>(&maps, shape);
 }
 
-struct Device { int sms, pairs; uint32_t *error; };          // pairs: clusters of two CTAs that fit at once
+// pairs: clusters of two CTAs of the pair loop that fit at once; clusters: of the other loop's, of 2, 4 and 8 CTAs
+struct Device { int sms, pairs, clusters[3]; uint32_t *error; };
 template <typename Kernel> bool AllowShared(Kernel *kernel)
 {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) == cudaSuccess) return true;
@@ -62,6 +63,10 @@ bool CurrentDevice(Device *d)
         cudaLaunchAttribute at[2];
         const cudaLaunchConfig_t cfg = LaunchConfig(at, v->sms / 2 * 2, 2, PairSmemBytes(kMaxExperts), nullptr);
         good = good && cudaOccupancyMaxActiveClusters(&v->pairs, Fp4GemmPairKernel<true>, &cfg) == cudaSuccess;
+        for (int i = 0; i < 3 && good; ++i) {
+            const cudaLaunchConfig_t c = LaunchConfig(at, v->sms / (2 << i) * (2 << i), 2 << i, 227 * 1024, nullptr);
+            good = cudaOccupancyMaxActiveClusters(&v->clusters[i], Fp4GemmKernel<true>, &c) == cudaSuccess;
+        }
         if (!good) cudaGetLastError();
         return good;
     });
@@ -103,8 +108,12 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 // us, single / pair: 500 x 3584 x 8192 13.7 / 15.1, 777 x 3584 x 8192 21.5 / 16.0, 256 x 8192 x 28672 34.8 / 41.1, 1024 x 1024 x 4096 9.0 / 10.0,
 // 2048 x 4096 x 1024 15.6 / 10.4, 4096 x 4096 x 4096 37.5 / 29.1, 8192 x 28672 x 8192 880 / 646; 32 experts, 7168 and 2048, gated and down: 64 rows
 // 66 / 81 and 37 / 53, 3000 95 / 112 and 60 / 67, 8000 142 / 140 and 107 / 89, 16000 237 / 225 and 180 / 144.
-struct Costs { double single, pair; };
-Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, int pairs)
+//
+// Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles fit at once and that is estimated to be
+// faster: exchanging sums takes 0.9 us, 0.2 a CTA and 12 ns a row.  us, alone / 2 / 4 / 8 of them: 1 x 4096 x 14336 15.0 / 10.6 / 9.5 / -,
+// 16 x 8192 x 28672 28.1 / 24.7 / - / -, 128 x 1024 x 4096 8.4 / 8.5 / 7.0 / 7.1, 16 x 8192 x 3584 6.8 / 7.6 / - / -, 16 x 4096 x 1024 3.8 / 4.5 / 5.2 / -.
+struct Costs { double single, pair; int split; };
+Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, int pairs, const int (&clusters)[3])
 {
     const double stages = (double)((K + kStageCols - 1) / kStageCols), matrices = experts > 0 ? std::min<double>((double)M, experts) : 1, rows = M / matrices;
     auto tiles = [&](double tall, double wide) {
@@ -113,9 +122,17 @@ Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, 
     };
     const double hbm = (17.0 / 32 * (M * K + matrices * (glu ? 2 : 1) * N * K) + 2.0 * M * N) / 6.5e6;
     const double used = std::min(rows, 128.0), stage = std::max(0.19, ((glu ? 2 : 1) * 17408 + 1024 + 128 * used) / 112e3);
-    const double single = std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 2.8 * used / 128);
     const double pair = std::ceil(tiles(256, glu ? 128 : 256) / std::max(pairs, 1)) * (stages * 0.34 + 1.5);
-    return {3.0 + std::max(single, hbm), 3.0 + std::max(pair, hbm)};
+    Costs c = {std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 2.8 * used / 128), pair, 1};
+    c.single = 3.0 + std::max(c.single, hbm) + 0.5;
+    c.pair = 3.0 + std::max(c.pair, hbm) + 0.5;
+    for (int i = 0; i < 3 && experts == 0; ++i) {
+        const int split = 2 << i;
+        if (tiles(128, 128) > clusters[i] || stages < split) continue;
+        const double us = 3.0 + std::max(std::ceil(stages / split) * stage, hbm) + 0.9 + 0.2 * split + 0.012 * used;
+        if (us < c.single) { c.single = us; c.split = split; }
+    }
+    return c;
 }
 
 // b[1] is the up projection of a gated product, else NULL.
@@ -146,7 +163,7 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     g.error = dev.error;
     const int matrices = std::max(experts, 1);
     const int64_t rowTiles = experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128;
-    const Costs costs = Estimate(M, N, K, experts, glu, dev.sms, dev.pairs);
+    const Costs costs = Estimate(M, N, K, experts, glu, dev.sms, dev.pairs, dev.clusters);
     const bool pairs = dev.pairs > 0 && M > 128 && costs.pair < costs.single;
     g.tilesN = pairs && !glu ? (N + 255) / 256 : (N + 127) / 128;
     g.group = pairs ? 8 : 16;
@@ -172,14 +189,15 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
         CHK_RET(ValueMap(&maps.b[h], b[h].values, matrices, N, K, 128));
         CHK_RET(ScaleMap(&maps.sb[h], b[h].scales, (int64_t)matrices * g.tileRowsB * g.tileCols));
     }
-    const int ctas = (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);
+    g.split = pairs ? 1 : costs.split;
+    const int ctas = g.split > 1 ? (int)(rowTiles * g.tilesN) * g.split : (int)std::min<int64_t>(dev.sms, rowTiles * g.tilesN);
     cudaError_t e;
     if (pairs) {
         const int both = 2 * (int)std::min<int64_t>(dev.pairs, rowTiles * g.tilesN);
         e = glu ? Launch(Fp4GemmPairKernel<true>, both, 2, PairSmemBytes(experts), stream, maps, g) : Launch(Fp4GemmPairKernel<false>, both, 2, PairSmemBytes(experts), stream, maps, g);
     } else {
-        e = glu ? Launch(Fp4GemmKernel<true>, ctas, 1, Config<256>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g)
-                : Launch(Fp4GemmKernel<false>, ctas, 1, Config<128>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g);
+        e = glu ? Launch(Fp4GemmKernel<true>, ctas, g.split, Config<256>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g)
+                : Launch(Fp4GemmKernel<false>, ctas, g.split, Config<128>::SmemBytes(g.aSlot, g.stages, experts), stream, maps, g);
     }
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -209,9 +227,12 @@ extern "C" int HcommFp4TakeError(void)
     if (v) cudaMemcpyToSymbol(g_error, &zero, sizeof(zero));
     return (int)v;
 }
-// What the rule makes of a product on a device of that many SMs and pairs of CTAs at once: us by single CTAs and by pairs.
-extern "C" void HcommToolFp4Estimate(int M, int N, int K, int experts, int gated, int sms, int pairs, double *us)
+// What the rule makes of a product on a device that holds so many SMs, pairs of CTAs and clusters of 2, 4 and 8 CTAs at once: us by single
+// CTAs and by pairs.  Returns how many single CTAs share a tile.
+extern "C" int HcommToolFp4Estimate(int M, int N, int K, int experts, int gated, int sms, int pairs, const int *clusters, double *us)
 {
-    const Costs c = Estimate(M, N, K, experts, gated != 0, sms, pairs);
+    const int held[3] = {clusters[0], clusters[1], clusters[2]};
+    const Costs c = Estimate(M, N, K, experts, gated != 0, sms, pairs, held);
     us[0] = c.single; us[1] = c.pair;
+    return c.split;
 }

@@ -22,12 +22,16 @@
 // Rows of A may be grouped by expert, with a matrix of B for each: tiles never cross a group; what a tile holds behind its
 // group's last row are other rows' values, which no stored value depends on.
 //
+// Where there are fewer tiles than SMs, the CTAs of a cluster share a tile along K.  Each leaves its sums in its own shared memory, where
+// all of them then read: every CTA adds up some of the tokens, over the CTAs in order, and stores them.
+//
 // A gated product (GLU) loads 128 rows of each of two matrices and keeps two accumulators, gate and up of the same element in the
 // same lane and thread, and stores silu(gate) * up.
 #pragma once
 #include <cuda_bf16.h>
 
 #include "fp4.cuh"
+#include "gemm_sm100_2sm.cuh"
 #include "sm100_ptx.cuh"
 
 namespace hcfp4 {
@@ -46,6 +50,7 @@ struct Shape {
     int group;                  // row tiles that are taken together before the next column of tiles
     int boxRows;                // rows of A that a load takes: a tile loads no more than it needs (one CTA a tile)
     int aSlot, stages;          // bytes of A in a stage; stages of the ring
+    int split;                  // CTAs of a cluster that share a tile along K
     int experts;                // 0: one matrix
     const int32_t *offsets;
     int tileCols, tileRowsB;    // tiles of scales along K; along N of one matrix
@@ -54,7 +59,7 @@ struct Shape {
     uint32_t *error;
 };
 
-constexpr int kMaxStages = 12;
+constexpr int kMaxStages = 12, kMaxSplit = 8;
 struct State {
     uint64_t full[kMaxStages], empty[kMaxStages], accFull[2], accEmpty[2];
     uint32_t tmem;
@@ -218,6 +223,60 @@ __device__ __forceinline__ void StoreTokens(const Shape &g, const Tile &t, uint3
     }
 }
 
+// Of a shared tile: the CTA's sums to shared memory, [gate, up][token][128 rows of weights] in 32 bits.
+template <bool GLU> __device__ __forceinline__ void KeepSums(const Tile &t, uint32_t accumulator, int warp, int lane, float *sums)
+{
+    const int q = warp & 3, first = (warp >> 2) * 64, tokens = t.rows - first;
+#pragma unroll
+    for (int h = 0; h < (GLU ? 2 : 1); ++h)
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+            if (tokens <= c) break;
+            uint32_t v[32];
+            TmemLoad32x32(accumulator + ((uint32_t)(q * 32) << 16) + h * 128 + first + c, v);
+            TmemLoadWait();
+            float *to = sums + ((h * 128 + first + c) * 128 + q * 32 + lane);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (c + j < tokens) to[j * 128] = __uint_as_float(v[j]);
+        }
+}
+__device__ __forceinline__ float2 LoadCluster(const float *p, int rank)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(hcgemm::pair::MapToCta(p, rank)) : "memory");
+    return v;
+}
+// All threads of all CTAs of the cluster, after everyone's sums are there.
+template <bool GLU> __device__ __forceinline__ void AddSums(const Shape &g, const Tile &t, const float *sums, int rank, bool pairs)
+{
+    const int n = (threadIdx.x & 63) * 2, column = t.column * 128 + n;
+    if (column >= g.N) return;
+    for (int token = rank + (threadIdx.x >> 6) * g.split; token < t.rows; token += kGemmThreads / 64 * g.split) {
+        float2 a[kMaxSplit], b[kMaxSplit];          // asked for all at once
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r) {
+            a[r] = b[r] = {0, 0};
+            if (r >= g.split) continue;
+            a[r] = LoadCluster(sums + token * 128 + n, r);
+            if constexpr (GLU) b[r] = LoadCluster(sums + (128 + token) * 128 + n, r);
+        }
+        float2 v = a[0], u = b[0];
+#pragma unroll
+        for (int r = 1; r < kMaxSplit; ++r) {
+            v.x += a[r].x; v.y += a[r].y;
+            if constexpr (GLU) { u.x += b[r].x; u.y += b[r].y; }
+        }
+        if constexpr (GLU) { v.x = SiluTimes(v.x, u.x); v.y = SiluTimes(v.y, u.y); }
+        __nv_bfloat16 *at = g.out + (int64_t)(t.row + token) * g.ldOut + column;
+        if (pairs && column + 1 < g.N) *(uint32_t *)at = Bf16Pair(v.x, v.y);
+        else {
+            at[0] = __float2bfloat16_rn(v.x);
+            if (column + 1 < g.N) at[1] = __float2bfloat16_rn(v.y);
+        }
+    }
+}
+
 template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, const Shape &g)
 {
     constexpr int BN = GLU ? 256 : 128;         // rows of weights: gate and up take 128 each
@@ -230,7 +289,11 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
     int *start = (int *)((uint8_t *)st + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stages = (g.K + kStageCols - 1) / kStageCols;
+    // a shared tile is the only one of its cluster
+    const int rank = g.split > 1 ? (int)hcgemm::pair::ClusterCtaRank() : 0, firstTile = g.split > 1 ? (int)blockIdx.x / g.split : (int)blockIdx.x;
+    const int tileStep = g.split > 1 ? 1 << 30 : (int)gridDim.x;
+    const int allStages = (g.K + kStageCols - 1) / kStageCols, firstStage = allStages * rank / g.split, endStage = allStages * (rank + 1) / g.split;
+    const bool pairs = g.ldOut % 2 == 0 && ((uintptr_t)g.out & 3) == 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < ring; ++s) { MbarInit(&st->full[s], 1); MbarInit(&st->empty[s], 1); }
         for (int a = 0; a < 2; ++a) { MbarInit(&st->accFull[a], 1); MbarInit(&st->accEmpty[a], kStoreWarps); }
@@ -259,12 +322,12 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
             int s = 0;
             uint32_t phase = 0;         // of the ring: flips each time round
             bool alive = true;
-            Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
+            Tiles<128> tiles(g, start, firstTile, tileStep, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
                 const int n = t.column * 128;
                 const int boxes = (t.rows + g.boxRows - 1) / g.boxRows, bytes = Cfg::StageBytes(boxes * g.boxRows * 128);
-                for (int k = 0; k < stages; ++k) {
+                for (int k = firstStage; k < endStage; ++k) {
                     if (!MbarWait(&st->empty[s], phase ^ 1, &st->abort)) { alive = false; break; }
                     uint8_t *a = smem + s * g.aSlot, *b = ringB + s * Cfg::kBBytes, *sa = ringSa + s * Cfg::kSaBytes, *sb = ringSb + s * Cfg::kSbBytes;
                     MbarExpectTx(&st->full[s], bytes);
@@ -289,7 +352,7 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
             uint32_t phase = 0, i = 0;
             const uint32_t lowA = DescLow(smem), lowB = DescLow(ringB), lowSa = DescLow(ringSa), lowSb = DescLow(ringSb);
             bool alive = true;
-            Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
+            Tiles<128> tiles(g, start, firstTile, tileStep, 0);
             Tile t;
             while (alive && tiles.Next(&t)) {
                 const uint32_t acc = i % Cfg::kAccumulators, accPhase = (i / Cfg::kAccumulators) & 1;
@@ -299,7 +362,7 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
                 const uint32_t d = tmem + acc * BN, tokens = (uint32_t)(t.rows + 15) / 16 * 16;
                 const uint32_t idesc[2] = {InstrDescMxf4(128, tokens, 0), InstrDescMxf4(128, tokens, 2)};
                 uint32_t more = 0;
-                for (int k = 0; k < stages; ++k) {
+                for (int k = firstStage; k < endStage; ++k) {
                     if (!MbarWait(&st->full[s], phase, &st->abort)) { alive = false; break; }
                     TcFenceAfter();
                     const uint32_t a = lowA + s * (g.aSlot >> 4), b = lowB + s * (Cfg::kBBytes >> 4), sa = lowSa + s * (Cfg::kSaBytes >> 4), sb = lowSb + s * (Cfg::kSbBytes >> 4);
@@ -330,9 +393,8 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
     } else if (warp >= 4) {
         // ------------------------------------------------------------------------------------ epilogue
         GridDependencyWait();
-        const bool pairs = g.ldOut % 2 == 0 && ((uintptr_t)g.out & 3) == 0;
         uint32_t i = 0;
-        Tiles<128> tiles(g, start, blockIdx.x, gridDim.x, 0);
+        Tiles<128> tiles(g, start, firstTile, tileStep, 0);
         Tile t;
         while (tiles.Next(&t)) {
             const uint32_t acc = i % Cfg::kAccumulators, phase = (i / Cfg::kAccumulators) & 1;
@@ -340,13 +402,21 @@ template <bool GLU> __device__ __forceinline__ void GemmLoop(const Maps *maps, c
             if (!MbarWait(&st->accFull[acc], phase, &st->abort)) break;
             __syncwarp();
             TcFenceAfter();
-            StoreTokens<GLU>(g, t, tmem + acc * BN, warp - 4, lane, pairs, [&] { MbarArrive(&st->accEmpty[acc]); });
+            if (g.split > 1) KeepSums<GLU>(t, tmem, warp - 4, lane, (float *)smem);
+            else StoreTokens<GLU>(g, t, tmem + acc * BN, warp - 4, lane, pairs, [&] { MbarArrive(&st->accEmpty[acc]); });
         }
     }
     // ---------------------------------------------------------------------------------------- the end
     TcFenceBefore();
     __syncthreads();
     TcFenceAfter();
+    if (g.split > 1) {
+        hcgemm::pair::ClusterSync();
+        GridDependencyWait();
+        Tile t;
+        if (Tiles<128>(g, start, firstTile, tileStep, 0).Next(&t)) AddSums<GLU>(g, t, (const float *)smem, rank, pairs);
+        hcgemm::pair::ClusterSync();            // nobody leaves while his sums are read
+    }
     if (warp == 1) TmemDealloc(tmem, 512);
     if (threadIdx.x == 0 && st->abort) atomicExch(g.error, 1u);
 }

@@ -14,7 +14,6 @@
 // A gated product has gate's 128 rows in the leader and up's in the other CTA.
 #pragma once
 #include "fp4_gemm.cuh"
-#include "gemm_sm100_2sm.cuh"
 
 namespace hcfp4 {
 

@@ -6,10 +6,14 @@ import pytest
 from hcomm_b200 import _lib
 
 
-def estimate(m, n, k, experts=0, gated=False, sms=148, pairs=74):
+def ask(m, n, k, experts=0, gated=False, sms=148, pairs=74, clusters=(74, 33, 15)):
     us = (ctypes.c_double * 2)()
-    _lib.load().HcommToolFp4Estimate(m, n, k, experts, int(gated), sms, pairs, us)
-    return list(us)
+    split = _lib.load().HcommToolFp4Estimate(m, n, k, experts, int(gated), sms, pairs, (ctypes.c_int * 3)(*clusters), us)
+    return split, list(us)
+
+
+def estimate(*shape):
+    return ask(*shape)[1]
 
 
 @pytest.mark.parametrize("shape", [(500, 3584, 8192), (256, 8192, 28672), (1024, 1024, 4096), (64, 7168, 2048, 32), (1000, 2048, 7168, 32, True), (5003, 2048, 7168, 32, True),
@@ -24,6 +28,19 @@ def test_single_ctas(shape):
 def test_pairs(shape):
     single, pair = estimate(*shape)
     assert pair < single
+
+
+@pytest.mark.parametrize("shape,splits", [((16, 8192, 28672), (2,)), ((1, 4096, 14336), (4,)), ((100, 4096, 14336), (4,)), ((1, 3584, 8192), (4,)), ((16, 8192, 3584), (1,)),
+                                          ((16, 4096, 4096), (2, 4)), ((128, 1024, 4096), (4, 8)), ((16, 4096, 1024), (1,)), ((16, 28672, 8192), (1,)), ((16, 136, 96), (1,)),
+                                          ((300, 1024, 4096), (4,))])
+def test_ctas_that_share_a_tile(shape, splits):
+    assert ask(*shape)[0] in splits
+
+
+def test_nothing_is_shared_where_clusters_do_not_fit():
+    assert ask(1, 4096, 14336, clusters=(31, 0, 0))[0] == 1 and ask(1, 4096, 14336, clusters=(32, 0, 0))[0] == 2
+    assert ask(8, 7168, 2048, 32)[0] == 1           # how many tiles there are is known on the device only
+    assert ask(1, 128, 512)[0] <= 2                 # never more CTAs than stages
 
 
 def test_estimates_are_near_what_was_measured():

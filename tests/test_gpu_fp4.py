@@ -284,3 +284,57 @@ def test_on_another_stream_and_in_a_replayed_graph():
     assert torch.equal(y, gemm_fp4(quantize_fp4(x), b))
     for e, (lo, hi) in enumerate(((0, 7), (7, 200))):
         check_gemm(out[lo:hi], nearest(x[lo:hi]), held(experts)[e])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 14336), (100, 1000, 4096), (16, 8192, 8192), (33, 130, 2080), (128, 1027, 5120), (200, 512, 8192)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_tiles_that_ctas_share_along_k(m, n, k, gated):
+    from hcomm_b200.ops.fp4 import gemm_fp4, gemm_fp4_swiglu, quantize_fp4
+    g = gen(m + n + k)
+    a = quantize_fp4(torch.randn(m, k, device="cuda", generator=g).to(torch.bfloat16))
+    b, up = (quantize_fp4(torch.randn(n, k, device="cuda", generator=g) * 0.02) for _ in range(2))
+    outs = [gemm_fp4_swiglu(a, b, up) if gated else gemm_fp4(a, b) for _ in range(3)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    if gated:
+        want, tol = swiglu_reference(held(a), held(b), held(up))
+        assert bool(((outs[0].double() - want).abs() <= tol).all())
+    else:
+        check_gemm(outs[0], held(a), held(b))
+    # an odd pitch: values one by one
+    big = torch.zeros(m, n + 3, device="cuda", dtype=torch.bfloat16)
+    (gemm_fp4_swiglu(a, b, up, big[:, 1:n + 1]) if gated else gemm_fp4(a, b, big[:, 1:n + 1]))
+    assert torch.equal(big[:, 1:n + 1], outs[0]) and not big[:, 0].any() and not big[:, n + 1:].any()
+
+
+def test_refusals():
+    from hcomm_b200.ops.fp4 import Fp4Tensor, dequantize_fp4, gemm_fp4, gemm_fp4_swiglu, quantize_fp4
+    torch.cuda.set_device(0)
+    x = torch.zeros(8, 128, device="cuda")
+    fp8, scales = x.to(torch.float8_e4m3fn), torch.ones(8, 1, device="cuda")
+    offsets = torch.tensor([0, 4, 8], device="cuda", dtype=torch.int32)
+    for error, args, kw in ((TypeError, (x.double(),), {}), (TypeError, (x.int(),), {}), (TypeError, (fp8,), {}), (TypeError, (x, scales), {}), (ValueError, (x[0],), {}),
+                            (ValueError, (x[:, :48],), {}), (ValueError, (x.t(),), {}), (ValueError, (fp8[:, :96], scales), {}), (ValueError, (fp8, scales[:4]), {}),
+                            (ValueError, (fp8, scales.double()), {}), (ValueError, (x.cpu(),), {}), (ValueError, (x,), dict(offsets=offsets.long())),
+                            (ValueError, (x,), dict(offsets=offsets[:1])), (ValueError, (x,), dict(offsets=offsets.cpu())), (ValueError, (x[None],), dict(offsets=offsets)),
+                            (ValueError, (x,), dict(offsets=torch.zeros(1026, device="cuda", dtype=torch.int32)))):
+        with pytest.raises(error):
+            quantize_fp4(*args, **kw)
+    q, w = quantize_fp4(x), quantize_fp4(torch.zeros(2, 16, 128, device="cuda"))
+    b, grouped = quantize_fp4(torch.zeros(16, 128, device="cuda")), quantize_fp4(x, offsets=offsets)
+    with pytest.raises(TypeError):
+        dequantize_fp4(q, torch.float8_e4m3fn)
+    with pytest.raises(ValueError):
+        dequantize_fp4(Fp4Tensor(q.values, q.scales[:0]))
+    wrong = quantize_fp4(torch.zeros(16, 96, device="cuda"))
+    out = torch.zeros(8, 16, device="cuda", dtype=torch.bfloat16)
+    for args in ((q, w), (grouped, b), (q, wrong), (q, grouped), (quantize_fp4(x, offsets=offsets[:2]), w), (w, b), (q, b, out.float()), (q, b, out[:, :8]), (q, b, out.t()),
+                 (q, b, out[:1].expand(8, 16)), (q, b, out.cpu()), (Fp4Tensor(q.values[:, ::2], q.scales), b), (q, Fp4Tensor(b.values, b.scales[:0]))):
+        with pytest.raises(ValueError):
+            gemm_fp4(*args)
+    with pytest.raises(TypeError):
+        gemm_fp4(x, b)
+    with pytest.raises(ValueError):
+        gemm_fp4_swiglu(q, b, quantize_fp4(torch.zeros(32, 128, device="cuda")))
+    assert gemm_fp4(quantize_fp4(x[:0]), b).shape == (0, 16)
+    with pytest.raises(ValueError):
+        gemm_fp4(quantize_fp4(x[:, :0]), quantize_fp4(torch.zeros(16, 0, device="cuda")))

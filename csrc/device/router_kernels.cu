@@ -16,6 +16,10 @@
 // lane among equals is the lowest index, and the k rounds of the choice are a maximum in the lane, one warp-wide integer
 // maximum (redux) and a ballot.  Sums over tokens stay in registers for as long as a warp works, then go to shared memory and, a
 // row for each block, to scratch; they are added up in a fixed order, so results do not depend on which block was first.
+//
+// What bounds it is the latency of a token's chain - maximum after maximum, then exponentials and sums across lanes - and beyond some
+// ten thousand tokens the instructions: us forward with counts and loss / backward, floor by bytes: 4096 x 256 bf16 11.6 / 5.8 (0.4, 0.7), 65003 x 64
+// fp32 34 / 20 (3, 6), 65536 x 256 fp32 70 / 47 (11, 21); 16 x 256 with a bias 6.0.  A token's row is asked for one token ahead (65536 x 256 fp32 backward 62 -> 47).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -24,13 +28,14 @@
 
 #include "../../include/hcomm_moe.h"
 #include "../core/log.h"
+#include "gemm_sm100_2sm.cuh"
 #include "sm100_ptx.cuh"
 
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopk = 16;
 constexpr uint32_t kAll = 0xffffffffu;
-constexpr int kFinishThreads = 1024;
+constexpr int kFinishThreads = 1024, kFinishCtas = 8;
 
 struct Params {
     const void *logits;
@@ -67,26 +72,28 @@ template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<8> { using type = uint2; };
 template <> struct Word<16> { using type = uint4; };
 
-// This lane's V values of a row; -inf behind the last expert.
-template <typename T, int V> __device__ __forceinline__ void LoadRow(float (&x)[V], const T *row, int experts, int first, bool vectors)
+// This lane's V values of a row as they lie in memory, asked for one token ahead of their use.
+template <typename T, int V> struct __align__(16) Raw { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ void AskRow(Raw<T, V> &raw, const T *row, int experts, int first, bool vectors)
 {
     constexpr int kBytes = V * (int)sizeof(T), kWord = kBytes > 16 ? 16 : kBytes;
     using W = typename Word<kWord>::type;
-    __align__(16) T raw[V];
     if (vectors) {
         if (first < experts) {
 #pragma unroll
-            for (int i = 0; i < kBytes / kWord; ++i) ((W *)raw)[i] = __ldg((const W *)(row + first) + i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = ToFloat(raw[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = -INFINITY;
+            for (int i = 0; i < kBytes / kWord; ++i) ((W *)raw.v)[i] = __ldg((const W *)(row + first) + i);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = first + j < experts ? ToFloat(row[first + j]) : -INFINITY;
+        for (int j = 0; j < V; ++j)
+            if (first + j < experts) raw.v[j] = row[first + j];
     }
+}
+// -inf behind the last expert
+template <typename T, int V> __device__ __forceinline__ void TakeRow(float (&x)[V], const Raw<T, V> &raw, int experts, int first)
+{
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = first + j < experts ? ToFloat(raw.v[j]) : -INFINITY;
 }
 template <typename T, int V> __device__ __forceinline__ void StoreRow(const float (&x)[V], T *row, int experts, int first, bool vectors)
 {
@@ -115,9 +122,9 @@ __device__ __forceinline__ float WarpSum(float v)
 }
 __device__ __forceinline__ float WarpMax(float v)
 {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
-    return v;
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
 // Integers that order like the floats they are made of, 0 for "not a candidate" (below every float).  Both zeros are one value.
@@ -131,6 +138,14 @@ __device__ __forceinline__ uint64_t Key(double x)
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return x == -INFINITY ? 0u : b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
 }
+// The same in the 16 bits of the type that x came from.
+template <typename T> __device__ __forceinline__ uint32_t Key16(float x);
+template <> __device__ __forceinline__ uint32_t Key16<__nv_bfloat16>(float x) { return Key(x) >> 16; }
+template <> __device__ __forceinline__ uint32_t Key16<__half>(float x)
+{
+    const uint32_t b = __half_as_ushort(__float2half_rn(x + 0.f));
+    return x == -INFINITY ? 0u : (b & 0x8000u ? ~b & 0xffffu : b | 0x8000u);
+}
 __device__ __forceinline__ uint32_t WarpMaxKey(uint32_t k) { return __reduce_max_sync(kAll, k); }
 __device__ __forceinline__ uint64_t WarpMaxKey(uint64_t k)
 {
@@ -142,33 +157,119 @@ __device__ __forceinline__ uint64_t WarpMaxKey(uint64_t k)
 // log sigmoid(x), also where the sigmoid itself is next to nothing
 __device__ __forceinline__ float LogSigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 
-// The k largest keys of the warp: lane i gets the i-th, its expert and its x; experts of -1 where no candidate is left.
-template <int V, typename K> __device__ __forceinline__ void TopK(K (&key)[V], const float (&x)[V], int topk, int lane, int *expert, float *value)
+__device__ __forceinline__ float Unkey(uint32_t k) { return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu)); }
+// Whether a <= b might be the other way round, see ChooseBiased.
+__device__ __forceinline__ bool Close(uint32_t upper, uint32_t lower)
 {
-    *expert = -1; *value = 0.f;
-    for (int i = 0; i < topk; ++i) {
+    const float a = Unkey(upper), b = Unkey(lower);
+    return !(a - b > 0x1p-20f * (1.f + fabsf(a) + fabsf(b)));
+}
+__device__ __forceinline__ bool Close(uint64_t, uint64_t) { return false; }
+
+// One step of the order inside a lane: the larger key first, of equal ones the one that stood in front.
+template <typename K> __device__ __forceinline__ void Order(K &a, K &b, uint32_t &ia, uint32_t &ib)
+{
+    const bool swap = b > a;
+    const K k = swap ? a : b;
+    const uint32_t i = swap ? ia : ib;
+    a = swap ? b : a; ia = swap ? ib : ia;
+    b = k; ib = i;
+}
+// The k largest keys of the warp: lane i gets the i-th's expert, -1 where no candidate is left; returns the largest key.  With close
+// it looks at one more and says whether two neighbours are.
+// Up to eight keys a lane are put in order first (by steps that keep equal ones in place), so that a round looks at one key a lane
+// and the winner moves its list up; places within the lane are four bits each of a word, which moves up with it.
+template <int V, typename K> __device__ __forceinline__ K TopK(K (&key)[V], int topk, int lane, int *expert, bool *close = nullptr)
+{
+    constexpr bool kSorted = V <= 8;
+    *expert = -1;
+    K largest = 0, before = 0;
+    uint32_t places = 0;
+    if constexpr (kSorted) {
+        uint32_t at[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) at[j] = j;
+#pragma unroll
+        for (int pass = 0; pass < V; ++pass)
+#pragma unroll
+            for (int j = pass & 1; j + 1 < V; j += 2) Order(key[j], key[j + 1], at[j], at[j + 1]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) places |= at[j] << 4 * j;
+    }
+    const int rounds = close ? topk + 1 : topk;
+    for (int i = 0; i < rounds; ++i) {
         K best = key[0];
-        int at = 0;
-        float bx = x[0];
+        int at = (int)(places & 15);
+        if constexpr (!kSorted) {
+            at = 0;
 #pragma unroll
-        for (int j = 1; j < V; ++j)
-            if (key[j] > best) { best = key[j]; at = j; bx = x[j]; }
+            for (int j = 1; j < V; ++j)
+                if (key[j] > best) { best = key[j]; at = j; }
+        }
         const K top = WarpMaxKey(best);
+        if (i == 0) largest = top;
         if (top == 0) break;
-        const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1;
-        const int e = __shfl_sync(kAll, lane * V + at, winner);
-        const float v = __shfl_sync(kAll, bx, winner);
-        if (lane == i) { *expert = e; *value = v; }
+        if (close && i) *close |= Close(before, top);
+        before = top;
+        const int winner = __ffs(__ballot_sync(kAll, best == top)) - 1, e = __shfl_sync(kAll, lane * V + at, winner);
+        if (lane == i && i < topk) *expert = e;
         if (lane == winner) {
+            if constexpr (kSorted) {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j == at) key[j] = 0;
+                for (int j = 0; j + 1 < V; ++j) key[j] = key[j + 1];
+                key[V - 1] = 0;
+                places >>= 4;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j == at) key[j] = 0;
+            }
         }
     }
+    return largest;
+}
+// The same of 16-bit keys, which share a word with the expert (the lower one is the larger word): no two words are equal, so that one
+// maximum says who it is.  (4096 tokens of 256 experts, bf16, choice alone: 10.0 us with keys of 32 bits, 9.6 so; 65536 of 128 experts 31 and 28.)
+template <int V> __device__ __forceinline__ uint32_t TopKPacked(uint32_t (&word)[V], int topk, int lane, int *expert)
+{
+    *expert = -1;
+    uint32_t largest = 0;
+    if constexpr (V <= 8) {
+#pragma unroll
+        for (int pass = 0; pass < V; ++pass)
+#pragma unroll
+            for (int j = pass & 1; j + 1 < V; j += 2) {
+                const uint32_t a = max(word[j], word[j + 1]), b = min(word[j], word[j + 1]);
+                word[j] = a; word[j + 1] = b;
+            }
+    }
+    for (int i = 0; i < topk; ++i) {
+        uint32_t best = word[0];
+        if constexpr (V > 8) {
+#pragma unroll
+            for (int j = 1; j < V; ++j) best = max(best, word[j]);
+        }
+        const uint32_t top = __reduce_max_sync(kAll, best);
+        if (i == 0) largest = top >> 16;
+        if (top >> 16 == 0) break;
+        if (lane == i) *expert = 0xffff - (int)(top & 0xffff);
+        if (best == top) {
+            if constexpr (V <= 8) {
+#pragma unroll
+                for (int j = 0; j + 1 < V; ++j) word[j] = word[j + 1];
+                word[V - 1] = 0;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (word[j] == top) word[j] = 0;
+            }
+        }
+    }
+    return largest;
 }
 
-// The row as probabilities: x becomes p; the row's maximum must not be -inf in all lanes.
-template <int V> __device__ __forceinline__ void Softmax(float (&x)[V], bool sigmoid)
+// The row as probabilities: x becomes p.  Logarithm of the largest score and 1 / sum, for a single score's own.
+template <int V> __device__ __forceinline__ float2 Softmax(float (&x)[V], bool sigmoid)
 {
     float top = -INFINITY;
 #pragma unroll
@@ -185,6 +286,7 @@ template <int V> __device__ __forceinline__ void Softmax(float (&x)[V], bool sig
     const float inverse = sum > 0 ? 1.f / sum : 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) x[j] *= inverse;
+    return {top, inverse};
 }
 
 // A row without a defined softmax (or sum of sigmoids): it holds a NaN, or +inf under softmax.
@@ -194,6 +296,32 @@ template <int V> __device__ __forceinline__ bool Undefined(const float (&x)[V], 
 #pragma unroll
     for (int j = 0; j < V; ++j) bad |= x[j] != x[j] || (!sigmoid && x[j] == INFINITY);
     return __any_sync(kAll, bad);
+}
+
+// The choice by sigmoid(x) + bias; true where a value is no number.  A choice between two scores that 32 bits cannot tell apart must not
+// hang on the way they were rounded, so it is made in 64 bits - but only for rows that need it, since an exponential in 64 bits costs as much as
+// everything else (65536 tokens, 256 experts: 124 us with all rows, 87 so).  In 32 bits a score is off by less than 2^-22, and by 2^-24 of the
+// sum with its bias: a row whose k + 1 best lie further apart than twice that has its order.
+template <int V> __device__ __forceinline__ bool ChooseBiased(const float (&x)[V], const Params &p, int first, int lane, int *expert)
+{
+    uint32_t quick[V];
+    float bias[V];
+    bool none = false, close = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        bias[j] = p.bias[first + j < p.experts ? first + j : 0];
+        const float s = x[j] == -INFINITY ? -INFINITY : 1.f / (1.f + expf(-x[j])) + bias[j];
+        none |= s != s;
+        quick[j] = Key(s);
+    }
+    if (__any_sync(kAll, none)) return true;
+    TopK<V, uint32_t>(quick, p.topk, lane, expert, &close);
+    if (!close) return false;
+    uint64_t key[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = Key(x[j] == -INFINITY ? (double)-INFINITY : 1.0 / (1.0 + exp(-(double)x[j])) + (double)bias[j]);
+    TopK<V, uint64_t>(key, p.topk, lane, expert);
+    return false;
 }
 
 // Share of the chosen: lanes below topk with an expert hold its x.
@@ -206,38 +334,27 @@ __device__ __forceinline__ float ChosenShare(float x, bool chosen, bool sigmoid)
     return chosen ? e / sum : 0.f;
 }
 
-// Adds up the blocks' rows of scratch (or takes the only block's sums), writes counts, sums and loss.  All threads of one block.
-__device__ void Finish(const Params &p, int blocks, const float *sums, const int32_t *counts, float *warpSum)
+__device__ __forceinline__ float Loss(const Params &p, float products, float tokens) { return p.balance * p.experts * (products / (tokens * p.topk) / tokens); }
+
+// A single block's sums are all there is: counts, sums and loss from shared memory.
+__device__ void FinishAlone(const Params &p, const float *sums, const int32_t *counts, float *warpSum)
 {
-    const int E = p.experts, threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __shared__ float total;
-    // the count of tokens lies behind those of the experts
-    if (warp == 0) {
-        int n = 0;
-        for (int b = lane; b < blocks; b += 32) n += counts[(size_t)b * (E + 1) + E];
-        n = __reduce_add_sync(kAll, n);
-        if (lane == 0) { p.counts[E] = n; total = (float)max(n, 1); }
-    }
-    float loss = 0;
-    for (int e = threadIdx.x; e < E; e += threads) {
-        int n = 0;
-        float s = 0;
-#pragma unroll 8
-        for (int b = 0; b < blocks; ++b) {
-            n += counts[(size_t)b * (E + 1) + e];
-            if (sums) s += sums[(size_t)b * E + e];
+    const int E = p.experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float products = 0;
+    for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+        p.counts[e] = counts[e];
+        if (e < E && sums) {
+            if (p.sums) p.sums[e] = sums[e];
+            products += (float)counts[e] * sums[e];
         }
-        p.counts[e] = n;
-        if (p.sums) p.sums[e] = s;
-        loss += (float)n * s;
     }
-    loss = WarpSum(loss);
-    if (lane == 0) warpSum[warp] = loss;
+    products = WarpSum(products);
+    if (lane == 0) warpSum[warp] = products;
     __syncthreads();
     if (threadIdx.x == 0 && p.loss) {
         float all = 0;
-        for (int w = 0; w < threads / 32; ++w) all += warpSum[w];
-        *p.loss = p.balance * E * (all / (total * p.topk) / total);
+        for (int w = 0; w < (int)blockDim.x / 32; ++w) all += warpSum[w];
+        *p.loss = Loss(p, all, (float)max(counts[E], 1));
     }
 }
 
@@ -261,55 +378,54 @@ __global__ void __launch_bounds__(Threads<V>()) RouteKernel(const __grid_constan
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] = 0;
     int seen = 0;
-    for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < p.tokens; t += (int64_t)gridDim.x * kWarps) {
-        const bool counted = !p.valid || p.valid[t];
+    const int64_t step = (int64_t)gridDim.x * kWarps;
+    int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+    Raw<T, V> next;
+    bool nextCounted = false;
+    auto ask = [&](int64_t t) {
+        if (t >= p.tokens) return;
+        AskRow<T, V>(next, (const T *)p.logits + t * p.ld, E, first, p.vectors);
+        nextCounted = !p.valid || p.valid[t];
+    };
+    ask(t);
+    for (; t < p.tokens; t += step) {
+        const bool counted = nextCounted;
+        float x[V];
+        TakeRow<T, V>(x, next, E, first);
+        ask(t + step);
         int expert = -1;
         float gate = 0;
         if (counted) {
             ++seen;
-            float x[V];
-            LoadRow<T, V>(x, (const T *)p.logits + t * p.ld, E, first, p.vectors);
-            bool bad = Undefined(x, p.sigmoid);
-            float value = 0;
-            if (p.bias) {
-                uint64_t key[V];
-                bool none = false;
+            const T *row = (const T *)p.logits + t * p.ld;
+            bool bad;
+            if (p.bias) bad = ChooseBiased<V>(x, p, first, lane, &expert);
+            else {
+                // a NaN, which an addition makes positive, has a key above that of infinity
+                uint32_t key[V], largest, infinity;
+                if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // in 64 bits: a choice between two scores that 32 bits cannot tell apart must not hang on the way they were rounded
-                    const double s = x[j] == -INFINITY ? -INFINITY : 1.0 / (1.0 + exp(-(double)x[j])) + (double)p.bias[first + j < E ? first + j : 0];
-                    none |= s != s;
-                    key[j] = Key(s);
+                    for (int j = 0; j < V; ++j) key[j] = Key16<T>(x[j]) << 16 | (0xffff - (uint32_t)(first + j));
+                    largest = TopKPacked<V>(key, p.topk, lane, &expert);
+                    infinity = Key16<T>(INFINITY);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) key[j] = Key(x[j]);
+                    largest = TopK<V, uint32_t>(key, p.topk, lane, &expert);
+                    infinity = Key(INFINITY);
                 }
-                bad = bad || __any_sync(kAll, none);
-                if (!bad) TopK<V, uint64_t>(key, x, p.topk, lane, &expert, &value);
-            } else {
-                uint32_t key[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) key[j] = Key(x[j]);
-                if (!bad) TopK<V, uint32_t>(key, x, p.topk, lane, &expert, &value);
+                bad = p.sigmoid ? largest > infinity : largest >= infinity;
             }
+            if (bad) expert = -1;
             const bool chosen = expert >= 0;
+            const float value = chosen ? ToFloat(row[expert]) : 0.f;
             if (p.renormalize) gate = ChosenShare(value, chosen, p.sigmoid);
             else if (p.sigmoid) gate = chosen ? expf(LogSigmoid(value)) : 0.f;
             if (stats || (!p.renormalize && !p.sigmoid)) {
-                float top = 0, whole = 0;
-                if (!p.renormalize && !p.sigmoid) {
-                    // the chosen one's probability from its own x, by the same steps as the row's
-                    top = -INFINITY;
+                const float2 s = Softmax(x, p.sigmoid);
+                if (!p.renormalize && !p.sigmoid) gate = chosen ? expf(value - s.x) * s.y : 0.f;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) top = fmaxf(top, x[j]);
-                    top = WarpMax(top);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) whole += x[j] == -INFINITY ? 0.f : expf(x[j] - top);
-                    whole = WarpSum(whole);
-                    gate = chosen ? expf(value - top) / whole : 0.f;
-                }
-                if (stats) {
-                    Softmax(x, p.sigmoid);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) sum[j] += bad ? NAN : x[j];
-                }
+                for (int j = 0; j < V; ++j) sum[j] += bad ? NAN : x[j];
             }
             gate = bad ? NAN : gate * p.scale;
             if (chosen) atomicAdd(&counts[expert], 1);
@@ -338,16 +454,58 @@ __global__ void __launch_bounds__(Threads<V>()) RouteKernel(const __grid_constan
         for (int e = threadIdx.x; e <= E; e += Threads<V>()) p.partCounts[(size_t)blockIdx.x * (E + 1) + e] = counts[e];
     } else {
         __syncthreads();
-        Finish(p, 1, stats ? rows : nullptr, counts, warpSum);
+        FinishAlone(p, stats ? rows : nullptr, counts, warpSum);
     }
 }
 
+// Adds up the blocks' rows of scratch (one CTA and a thread for each expert took 10 us of 23 at 4096 tokens): a cluster of eight CTAs, each with an eighth of the experts and as many groups of threads as
+// there is room for, each with some of the blocks.  Every sum goes through its blocks, then its groups, then its CTAs in order.
 __global__ void __launch_bounds__(kFinishThreads) FinishKernel(const __grid_constant__ Params p, int blocks)
 {
-    __shared__ float warpSum[32];
+    __shared__ float groupSum[kFinishThreads], products[kFinishThreads / 32], mine;
+    __shared__ int32_t groupCount[kFinishThreads];
     sm100::GridDependencyWait();
     sm100::GridDependentsLaunch();
-    Finish(p, blocks, p.partSums, p.partCounts, warpSum);
+    const int E = p.experts, rank = (int)hcgemm::pair::ClusterCtaRank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int width = (E + 1 + kFinishCtas - 1) / kFinishCtas, groups = kFinishThreads / width, group = threadIdx.x / width, in = threadIdx.x % width, e = rank * width + in;
+    int n = 0;
+    float s = 0;
+    if (group < groups && e <= E) {
+#pragma unroll 8
+        for (int b = group; b < blocks; b += groups) {
+            n += p.partCounts[(size_t)b * (E + 1) + e];
+            if (p.partSums && e < E) s += p.partSums[(size_t)b * E + e];
+        }
+    }
+    groupCount[threadIdx.x] = n; groupSum[threadIdx.x] = s;
+    __syncthreads();
+    float product = 0;
+    if (threadIdx.x < width && e <= E) {
+        for (int g = 1; g < groups; ++g) { n += groupCount[g * width + in]; s += groupSum[g * width + in]; }
+        p.counts[e] = n;
+        if (e < E) {
+            if (p.sums) p.sums[e] = s;
+            product = (float)n * s;
+        } else groupCount[0] = n;           // of tokens: the last CTA's, no other thread of which still reads its group's first entry
+    }
+    product = WarpSum(product);
+    if (lane == 0) products[warp] = product;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        mine = 0;
+        for (int w = 0; w < kFinishThreads / 32; ++w) mine += products[w];
+    }
+    hcgemm::pair::ClusterSync();
+    if (rank == E / width && threadIdx.x == 0 && p.loss) {
+        float all = 0;
+        for (int r = 0; r < kFinishCtas; ++r) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(hcgemm::pair::MapToCta(&mine, r)) : "memory");
+            all += v;
+        }
+        *p.loss = Loss(p, all, (float)max(groupCount[0], 1));
+    }
+    hcgemm::pair::ClusterSync();            // nobody leaves while his sum is read
 }
 
 // The loss from counts and sums that were added up over ranks: one warp.
@@ -383,25 +541,35 @@ __global__ void __launch_bounds__(Threads<V>()) RouteBackwardKernel(const __grid
         for (int j = 0; j < V; ++j) w[j] = 0;
     }
     __syncwarp();
-    for (int64_t t = (int64_t)blockIdx.x * kWarps + warp; t < p.tokens; t += (int64_t)gridDim.x * kWarps) {
-        float d[V];
-        if (p.valid && !p.valid[t]) {
+    const int64_t step = (int64_t)gridDim.x * kWarps;
+    int64_t t = (int64_t)blockIdx.x * kWarps + warp;
+    Raw<T, V> next;
+    bool nextCounted = false;
+    int nextExpert = -1;
+    float nextGrad = 0;
+    auto ask = [&](int64_t t) {
+        if (t >= p.tokens) return;
+        AskRow<T, V>(next, (const T *)p.logits + t * p.ld, E, first, p.vectors);
+        nextCounted = !p.valid || p.valid[t];
+        if (p.dgates && lane < p.topk) {
+            nextExpert = p.idx[t * p.topk + lane];
+            nextGrad = p.dgates[t * p.topk + lane];
+        }
+    };
+    ask(t);
+    for (; t < p.tokens; t += step) {
+        const bool counted = nextCounted;
+        int expert = nextExpert < E ? nextExpert : -1;
+        const float grad = nextGrad;
+        float x[V], d[V];
+        TakeRow<T, V>(x, next, E, first);
+        ask(t + step);
+        if (!counted) {
 #pragma unroll
             for (int j = 0; j < V; ++j) d[j] = 0;
         } else {
-            const T *row = (const T *)p.logits + t * p.ld;
-            float x[V];
-            LoadRow<T, V>(x, row, E, first, p.vectors);
             const bool bad = Undefined(x, p.sigmoid);
-            int expert = -1;
-            float dg = 0, value = 0;
-            if (p.dgates && lane < p.topk) {
-                expert = p.idx[t * p.topk + lane];
-                if (expert >= 0 && expert < E) {
-                    dg = p.dgates[t * p.topk + lane] * p.scale;
-                    value = ToFloat(row[expert]);
-                } else expert = -1;
-            }
+            const float dg = expert >= 0 ? grad * p.scale : 0.f, value = expert >= 0 ? ToFloat(((const T *)p.logits)[t * p.ld + expert]) : 0.f;
             const bool chosen = expert >= 0;
             float to = dg;                      // to the chosen expert alone
             if (p.renormalize) {
@@ -461,7 +629,8 @@ int BlocksOf(int tokens, int experts, int sms)
 }
 constexpr int kMostBlocks = 256;        // of scratch, whatever the device
 
-template <typename Kernel, typename... Args> HcclResult Launch(const char *what, Kernel *kernel, int grid, int threads, int smem, void *stream, const Args &...args)
+template <typename Kernel, typename... Args>
+HcclResult Launch(const char *what, Kernel *kernel, int grid, int cluster, int threads, int smem, void *stream, const Args &...args)
 {
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         HCCL_ERROR("%s: %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
@@ -472,10 +641,12 @@ template <typename Kernel, typename... Args> HcclResult Launch(const char *what,
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -489,7 +660,7 @@ template <typename T, bool BACKWARD> HcclResult LaunchRows(const char *what, con
     const int v = ValuesOf(p.experts), warps = WarpsOf(v);
     const int smem = BACKWARD ? warps * 32 * v * 4 : 4 * (p.experts + 1 + (p.partSums ? warps * p.experts : 0));
     switch (v) {
-#define HCOMM_CASE(V) case V: return Launch(what, BACKWARD ? RouteBackwardKernel<T, V> : RouteKernel<T, V>, grid, warps * 32, smem, stream, p);
+#define HCOMM_CASE(V) case V: return Launch(what, BACKWARD ? RouteBackwardKernel<T, V> : RouteKernel<T, V>, grid, 1, warps * 32, smem, stream, p);
         HCOMM_CASE(1) HCOMM_CASE(2) HCOMM_CASE(4) HCOMM_CASE(8) HCOMM_CASE(16) HCOMM_CASE(32)
 #undef HCOMM_CASE
     }
@@ -553,7 +724,7 @@ extern "C" int HcommMoeRoute(const void *logits, int dataType, int64_t ldLogits,
     p.partSums = stats ? (blocks > 1 ? (float *)scratch : (float *)counts) : nullptr;
     p.partCounts = (int32_t *)scratch + (blocks > 1 ? (size_t)blocks * experts : 0);
     CHK_RET(LaunchTyped<false>("HcommMoeRoute", p, dataType, blocks, stream));
-    if (blocks > 1) return Launch("HcommMoeRoute", FinishKernel, 1, kFinishThreads, 0, stream, p, blocks);
+    if (blocks > 1) return Launch("HcommMoeRoute", FinishKernel, kFinishCtas, kFinishCtas, kFinishThreads, 0, stream, p, blocks);
     return HCCL_SUCCESS;
 }
 
@@ -564,7 +735,7 @@ extern "C" int HcommMoeBalanceLoss(const int32_t *counts, const float *probSums,
         return HCCL_E_PARA;
     }
     if (!counts || !probSums || !loss) return HCCL_E_PTR;
-    return Launch("HcommMoeBalanceLoss", BalanceLossKernel, 1, 32, 0, stream, counts, probSums, experts, topk, balance, loss);
+    return Launch("HcommMoeBalanceLoss", BalanceLossKernel, 1, 1, 32, 0, stream, counts, probSums, experts, topk, balance, loss);
 }
 
 extern "C" int HcommMoeRouteBackward(const void *logits, int dataType, int64_t ldLogits, int tokens, int experts, int topk, int scoring, int renormalize, float scale, const uint8_t *valid,

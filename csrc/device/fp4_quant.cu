@@ -24,6 +24,7 @@ namespace {
 using namespace hcfp4;
 
 constexpr int kThreads = 256;
+constexpr int64_t kMostRows = INT32_MAX - (1 << 20);       // a step behind the last row is still a 32-bit number
 
 struct Rows {
     int64_t rows, cols;                     // of one matrix
@@ -322,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) DequantizeKernel(Rows r
 
 HcclResult CheckRows(const char *what, int64_t batch, int64_t rows, int64_t cols, const int32_t *offsets, int experts)
 {
-    if (batch < 0 || rows < 0 || cols < 0 || cols % kBlock || rows > INT32_MAX || cols > INT32_MAX || (batch && rows > INT32_MAX / batch)) {
-        RPT_ERR("EI0003", "%s: %lld x %lld x %lld, columns must be a multiple of 32 and rows fewer than 2^31 in all", what, (long long)batch, (long long)rows, (long long)cols);
+    if (batch < 0 || rows < 0 || cols < 0 || cols % kBlock || rows > INT32_MAX || cols > INT32_MAX || (batch && rows > kMostRows / batch)) {
+        RPT_ERR("EI0003", "%s: %lld x %lld x %lld, columns must be a multiple of 32 and rows no more than 2^31 - 2^20 in all", what, (long long)batch, (long long)rows, (long long)cols);
         return HCCL_E_PARA;
     }
     if (experts < 0 || experts > kMaxExperts || (experts > 0) != (offsets != nullptr) || (experts > 0 && batch != 1)) {
@@ -383,8 +384,8 @@ extern "C" int HcommFp4Quantize(const void *x, int dataType, const float *xScale
     const bool fp8 = dataType == HCCL_DATA_TYPE_FP8E4M3;
     if (batch * rows * cols == 0) return HCCL_SUCCESS;
     if (!x || !values || !scales || (fp8 && !xScales)) return HCCL_E_PTR;
-    if (rowPitch < cols || batchPitch < 0 || ((uintptr_t)values & 15) || ((uintptr_t)scales & 15) || (fp8 && (cols % 128 || scalePitch < cols / 128 || batch != 1))) {
-        RPT_ERR("EI0003", "HcommFp4Quantize: row pitch %lld of %lld columns, scale pitch %lld; outputs must be 16-byte aligned, fp8 rows a multiple of 128 wide and one matrix",
+    if (rowPitch < 0 || batchPitch < 0 || ((uintptr_t)values & 15) || ((uintptr_t)scales & 15) || (fp8 && (cols % 128 || scalePitch < 0 || batch != 1))) {
+        RPT_ERR("EI0003", "HcommFp4Quantize: row pitch %lld of %lld columns, scale pitch %lld (none negative); outputs must be 16-byte aligned, fp8 rows a multiple of 128 wide and one matrix",
                 (long long)rowPitch, (long long)cols, (long long)scalePitch);
         return HCCL_E_PARA;
     }

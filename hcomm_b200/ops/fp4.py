@@ -53,9 +53,12 @@ class Fp4Tensor:
         if values.shape[:-1] != scales.shape[:-1] or values.shape[-1] != 16 * scales.shape[-1] or values.device != scales.device:
             raise ValueError(f"values {tuple(values.shape)} and scales {tuple(scales.shape)} do not belong together")
         rows, blocks = scales.shape[-2:]
-        s = torch.nn.functional.pad(scales.reshape(-1, rows, blocks), (0, -blocks % 4, 0, -rows % 128))
+        s = scales.reshape(-1, rows, blocks)
+        if blocks % 4 or rows % 128:
+            s = torch.nn.functional.pad(s, (0, -blocks % 4, 0, -rows % 128))
         s = s.view(s.shape[0], s.shape[1] // 128, 4, 32, s.shape[2] // 4, 4).permute(0, 1, 4, 3, 2, 5)
-        return cls(values.contiguous(), s.reshape(-1, 512).contiguous())
+        values = values.contiguous()
+        return cls(values if values.data_ptr() % 16 == 0 else values.clone(), s.reshape(-1, 512).contiguous())
 
     def block_scales(self) -> torch.Tensor:
         """The scales as ``from_parts`` takes them, [..., rows, cols // 32]; not of grouped rows."""

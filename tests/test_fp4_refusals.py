@@ -43,8 +43,8 @@ def quantize(x=64, kind=_lib.BF16, xs=0, batch=1, rows=4, cols=64, batch_pitch=0
 
 
 def test_quantise_refuses():
-    for bad in (dict(cols=48), dict(cols=-32), dict(rows=-1), dict(rows=1 << 31), dict(row_pitch=32), dict(values=72), dict(scales=72), dict(kind=_lib.FP64), dict(kind=_lib.INT8),
-                dict(kind=_lib.FP8E4M3, xs=64), dict(kind=_lib.FP8E4M3, xs=64, cols=128, row_pitch=128), dict(kind=_lib.FP8E4M3, xs=64, cols=128, row_pitch=128, batch=2, scale_pitch=1),
+    for bad in (dict(cols=48), dict(cols=-32), dict(rows=-1), dict(rows=1 << 31), dict(rows=(1 << 31) - 1), dict(batch=1 << 20, rows=1 << 11), dict(row_pitch=-1), dict(batch_pitch=-1, batch=2), dict(values=72), dict(scales=72), dict(kind=_lib.FP64), dict(kind=_lib.INT8),
+                dict(kind=_lib.FP8E4M3, xs=64), dict(kind=_lib.FP8E4M3, xs=64, cols=128, row_pitch=128, scale_pitch=-1), dict(kind=_lib.FP8E4M3, xs=64, cols=128, row_pitch=128, batch=2, scale_pitch=1),
                 dict(experts=2), dict(offsets=64), dict(offsets=64, experts=1025), dict(offsets=64, experts=2, batch=2), dict(experts=-1)):
         assert quantize(**bad) == PARA, bad
     for bad in (dict(x=0), dict(values=0), dict(scales=0), dict(kind=_lib.FP8E4M3, cols=128, row_pitch=128, scale_pitch=1)):
@@ -70,7 +70,7 @@ def test_products_refuse():
         fn = _lib.load().HcommFp4GemmSwiglu if gated else _lib.load().HcommFp4Gemm
         return fn(*[p(o) for o in ops[:6 if gated else 4]], p(out), m, n, k, i64(ld), p(offsets), experts, p(0))
     for gated in (False, True):
-        for bad in (dict(k=48), dict(k=0), dict(m=-1), dict(n=-1), dict(ld=7), dict(experts=2), dict(offsets=64), dict(offsets=64, experts=1025), dict(out=65),
+        for bad in (dict(k=48), dict(k=0), dict(m=-1), dict(n=-1), dict(m=(1 << 31) - 1), dict(n=(1 << 31) - 1, ld=1 << 31), dict(ld=7), dict(experts=2), dict(offsets=64), dict(offsets=64, experts=1025), dict(out=65),
                     dict(ops=(72, 64, 64, 64, 64, 64)), dict(ops=(64, 64, 64, 72, 64, 64))):
             assert call(gated=gated, **bad) == PARA, bad
         for bad in (dict(out=0), dict(ops=(0, 64, 64, 64, 64, 64)), dict(ops=(64, 64, 64, 0, 64, 64))):

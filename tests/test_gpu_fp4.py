@@ -124,6 +124,8 @@ def test_strides_alignment_and_several_matrices():
         for x in (cube, cube[::2], cube[:, 1:, :96], cube.transpose(0, 1), cube[:1]):
             q = quantize_fp4(x)
             assert same(held(q), nearest(x)) and same(dequantize_fp4(q, torch.float32), nearest(x))
+    row = spread(g, 1, 96)
+    assert same(held(quantize_fp4(row.expand(70, 96))), nearest(row).expand(70, 96))
     for shape in ((0, 64), (4, 0), (0, 3, 32), (2, 0, 32)):
         q = quantize_fp4(torch.empty(shape, device="cuda"))
         assert q.shape == shape and dequantize_fp4(q).shape == shape
@@ -338,3 +340,65 @@ def test_refusals():
     assert gemm_fp4(quantize_fp4(x[:0]), b).shape == (0, 16)
     with pytest.raises(ValueError):
         gemm_fp4(quantize_fp4(x[:, :0]), quantize_fp4(torch.zeros(16, 0, device="cuda")))
+
+
+def test_a_checkpoint_that_is_not_aligned():
+    from hcomm_b200.ops.fp4 import Fp4Tensor, gemm_fp4, quantize_fp4
+    g = gen(51)
+    codes = torch.randint(0, 256, (1 + 40 * 48,), device="cuda", generator=g, dtype=torch.uint8)[1:].view(40, 48)
+    w = Fp4Tensor.from_parts(codes, torch.randint(120, 130, (40, 3), device="cuda", generator=g, dtype=torch.uint8))
+    a = quantize_fp4(spread(g, 5, 96))
+    check_gemm(gemm_fp4(a, w), held(a), held(w))
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from hcomm_b200.ops.fp4 import gemm_fp4, quantize_fp4
+from hcomm_b200.ops.router import route
+x = torch.randn({m}, 512, device="cuda").to(torch.bfloat16)
+w = torch.randn(2048, 512, device="cuda").to(torch.bfloat16)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = gemm_fp4(quantize_fp4(x), quantize_fp4(w))
+    r = route(y[:, :64], 4)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, gemm_fp4(quantize_fp4(x), quantize_fp4(w))) and torch.equal(r.topk_idx, route(y[:, :64], 4).topk_idx)
+print("same")
+"""
+
+
+@pytest.mark.parametrize("m", [20, 6000])
+def test_first_calls_of_a_process_are_captured(m):
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parent.parent)
+    res = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=root, m=m)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "same" in res.stdout, res.stdout + res.stderr
+
+
+def test_threads_and_streams_at_the_same_time():
+    import threading
+    from hcomm_b200.ops.fp4 import gemm_fp4, quantize_fp4, take_kernel_error
+    g = gen(61)
+    w = weights(g, 1024, 1024)
+    xs = [torch.randn(m, 1024, device="cuda", generator=g).to(torch.bfloat16) for m in (1, 40, 300, 2000)]
+    want = [gemm_fp4(quantize_fp4(x), w) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        torch.cuda.set_device(0)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(gemm_fp4(quantize_fp4(xs[i]), w), want[i]):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and take_kernel_error() == 0

@@ -60,6 +60,7 @@ struct Shape {
 };
 
 constexpr int kMaxStages = 12, kMaxSplit = 8;
+constexpr int kRoom = 224 * 1024;           // of shared memory: leaves a small block of the kernel in front its place
 struct State {
     uint64_t full[kMaxStages], empty[kMaxStages], accFull[2], accEmpty[2];
     uint32_t tmem;
@@ -82,7 +83,7 @@ template <int BN> struct Config {
     static constexpr int StageBytes(int aSlot) { return aSlot + kBBytes + kSaBytes + kSbBytes; }
     static constexpr int Stages(int aSlot, int experts)
     {
-        const int room = 227 * 1024 - 1024 - kTail - (experts > 0 ? 4 * (experts + 1) : 0), fit = room / StageBytes(aSlot), columns = (512 - kScaleBase) / kScaleCols;
+        const int room = kRoom - 1024 - kTail - (experts > 0 ? 4 * (experts + 1) : 0), fit = room / StageBytes(aSlot), columns = (512 - kScaleBase) / kScaleCols;
         return fit < columns ? (fit < kMaxStages ? fit : kMaxStages) : (columns < kMaxStages ? columns : kMaxStages);
     }
     static constexpr int SmemBytes(int aSlot, int stages, int experts) { return 1024 + stages * StageBytes(aSlot) + kTail + (experts > 0 ? 4 * (experts + 1) : 0); }

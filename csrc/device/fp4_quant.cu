@@ -178,7 +178,8 @@ template <typename T> constexpr int kBlocks = sizeof(T) == 1 ? 3 : 5;           
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocks<T>) QuantizeKernel(Rows r, Source s, uint8_t *values, uint8_t *scales)
 {
-    __shared__ int start[kMaxExperts + 1], tile[kMaxExperts + 1];
+    extern __shared__ int start[];          // with grouped rows: where each expert's start, then where its tiles do
+    int *const tile = start + r.experts + 1;
     sm100::GridDependencyWait();
     sm100::GridDependentsLaunch();
     const Range range = RowsOf(r, start, tile);
@@ -283,7 +284,8 @@ constexpr int kBlocksBack = 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads, kBlocksBack) DequantizeKernel(Rows r, const uint8_t *values, const uint8_t *scales, T *out)
 {
-    __shared__ int start[kMaxExperts + 1], tile[kMaxExperts + 1];
+    extern __shared__ int start[];          // with grouped rows: where each expert's start, then where its tiles do
+    int *const tile = start + r.experts + 1;
     sm100::GridDependencyWait();
     sm100::GridDependentsLaunch();
     const Range range = RowsOf(r, start, tile);
@@ -335,7 +337,7 @@ HcclResult CheckRows(const char *what, int64_t batch, int64_t rows, int64_t cols
 }
 
 // Programmatic launch: set-up overlaps the end of the kernel in front, which the kernel waits for before it touches memory.
-template <typename... Params, typename... Args> HcclResult Launch(const char *what, void (*kernel)(Params...), int64_t chunks, int lanes, int blocks, void *stream, Args... args)
+template <typename... Params, typename... Args> HcclResult Launch(const char *what, void (*kernel)(Params...), int64_t chunks, int lanes, int blocks, int experts, void *stream, Args... args)
 {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -345,6 +347,7 @@ template <typename... Params, typename... Args> HcclResult Launch(const char *wh
     const int teams = kThreads / lanes;
     cfg.gridDim = dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((chunks + teams - 1) / teams, (int64_t)sms * blocks)), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = experts > 0 ? 8 * (experts + 1) : 0;         // no more, so that a product behind finds room beside the last blocks
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -361,11 +364,11 @@ template <typename... Params, typename... Args> HcclResult Launch(const char *wh
 template <typename T>
 HcclResult LaunchQuantize(const Rows &r, const Source &s, void *values, void *scales, void *stream)
 {
-    return Launch("HcommFp4Quantize", QuantizeKernel<T>, r.batch * r.rows * r.tileCols, kLanes<T>, kBlocks<T>, stream, r, s, (uint8_t *)values, (uint8_t *)scales);
+    return Launch("HcommFp4Quantize", QuantizeKernel<T>, r.batch * r.rows * r.tileCols, kLanes<T>, kBlocks<T>, r.experts, stream, r, s, (uint8_t *)values, (uint8_t *)scales);
 }
 template <typename T> HcclResult LaunchDequantize(const Rows &r, const void *values, const void *scales, void *out, void *stream)
 {
-    return Launch("HcommFp4Dequantize", DequantizeKernel<T>, r.batch * r.rows * r.tileCols, 8, kBlocksBack, stream, r, (const uint8_t *)values, (const uint8_t *)scales, (T *)out);
+    return Launch("HcommFp4Dequantize", DequantizeKernel<T>, r.batch * r.rows * r.tileCols, 8, kBlocksBack, r.experts, stream, r, (const uint8_t *)values, (const uint8_t *)scales, (T *)out);
 }
 
 }  // namespace

@@ -8,6 +8,7 @@
     python -m hcomm_b200.utils.profile_cases fused_pair      the CTA-pair variants of the two fused kernels on a one-rank communicator
     python -m hcomm_b200.utils.profile_cases moe             MoE dispatch + combine, one rank (256 experts, top-8, hidden 7168)
     python -m hcomm_b200.utils.profile_cases single          kernels of the single-GPU cases: the plain GEMM at five shapes, MoE, a scaled copy (two rounds of eight)
+    python -m hcomm_b200.utils.profile_cases experts         routing forward and backward, 4-bit quantisation and products: few rows, one rank's experts, many rows (two rounds of fourteen)
 
 Ranks that share the GPU run inside ONE cooperative launch (kernels that wait for each other are never separate
 launches on a GPU), so each case is a single process a profiler can wrap.  A few launches per kernel, a few hundred
@@ -199,10 +200,37 @@ def case_single(reps=2):
     comm.destroy()
 
 
+def case_experts(reps=2):
+    """Two rounds of: routing of 4096 tokens (256 experts, 8 each) with its loss, and its gradient; a weight quantised and back; a
+    product of 16 rows, of one row whose tiles are shared along K, and of 4096; 32 experts' gate and up products and down product for 512 and for
+    8192 fp8 rows.  1 GB on the device."""
+    from ..ops.fp4 import dequantize_fp4, gemm_fp4, gemm_fp4_swiglu, quantize_fp4, take_kernel_error
+    from ..ops.moe import quantize_e4m3_1x128
+    from ..ops.router import route
+    logits = torch.randn(4096, 256, device="cuda").to(torch.bfloat16).requires_grad_()
+    weight = torch.randn(8192, 8192, device="cuda").to(torch.bfloat16)
+    big, deep = quantize_fp4(torch.randn(28672, 8192, device="cuda").to(torch.bfloat16)), quantize_fp4(torch.randn(4096, 14336, device="cuda").to(torch.bfloat16))
+    acts = [quantize_fp4(torch.randn(m, k, device="cuda").to(torch.bfloat16)) for m, k in ((16, 8192), (1, 14336), (4096, 8192))]
+    gate, up, down = (quantize_fp4((torch.randn(32, n, k, device="cuda") * 0.02).to(torch.bfloat16)) for n, k in ((2048, 7168), (2048, 7168), (7168, 2048)))
+    rows = [(*quantize_e4m3_1x128(torch.randn(r, 7168, device="cuda")), torch.arange(0, r + 1, r // 32, device="cuda", dtype=torch.int32)) for r in (512, 8192)]
+    for _ in range(reps):
+        r = route(logits, 8, balance=0.01)
+        torch.autograd.grad((r.gates.sum(), r.loss), logits)
+        dequantize_fp4(quantize_fp4(weight))
+        gemm_fp4(acts[0], big)
+        gemm_fp4(acts[1], deep)
+        gemm_fp4(acts[2], big)
+        for x, scales, offsets in rows:
+            h = gemm_fp4_swiglu(quantize_fp4(x, scales, offsets=offsets), gate, up)
+            gemm_fp4(quantize_fp4(h, offsets=offsets), down)
+    torch.cuda.synchronize()
+    assert take_kernel_error() == 0
+
+
 def main():
     torch.cuda.set_device(0)
     which = sys.argv[1] if len(sys.argv) > 1 else "gemm"
-    {"gemm": case_gemm, "gemm_up": case_gemm_up, "gemm_raster": case_gemm_raster, "fused": case_fused, "fused_pair": case_fused_pair, "allreduce": case_allreduce, "moe": case_moe, "single": case_single}[which]()
+    {"gemm": case_gemm, "gemm_up": case_gemm_up, "gemm_raster": case_gemm_raster, "fused": case_fused, "fused_pair": case_fused_pair, "allreduce": case_allreduce, "moe": case_moe, "single": case_single, "experts": case_experts}[which]()
     print(f"profile case {which}: done", flush=True)
 
 

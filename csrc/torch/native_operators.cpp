@@ -6,8 +6,10 @@
 #include "plain.h"
 
 #include <ATen/ops/empty.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include "released.h"
 
@@ -15,7 +17,7 @@ namespace {
 
 using namespace hcomm_torch;
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using QuantizeFn = int (*)(const void *, int, const float *, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, const int32_t *, int, void *, void *, void *);
 using DequantizeFn = int (*)(const void *, const void *, int64_t, int64_t, int64_t, const int32_t *, int, void *, int, void *);
@@ -193,46 +195,62 @@ Routed Forward(const RouteCall &c, const Tensor &x)
     return r;
 }
 
-struct RouteNode : public torch::autograd::Function<RouteNode> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &x, const RouteCall *c, int *rc)
+// The routing in the autograd graph: inputs of the node are the gradients of gates and loss, its output that of the logits.
+struct RouteNode : public torch::autograd::Node {
+    SavedVariable x, valid, idx, counts;
+    RouteBackwardFn backward;
+    int topk, scoring, renormalize;
+    float scale, balance;
+
+    variable_list apply(variable_list &&grads) override
     {
-        Routed r = Forward(*c, x);
-        *rc = r.rc;
-        ctx->save_for_backward({x, c->valid ? *c->valid : Tensor(), r.idx, r.counts});
-        ctx->saved_data["entry"] = (int64_t)(uintptr_t)c->backward;
-        ctx->saved_data["scoring"] = (int64_t)c->scoring;
-        ctx->saved_data["renormalize"] = (int64_t)c->renormalize;
-        ctx->saved_data["scale"] = (double)c->scale;
-        ctx->saved_data["balance"] = (double)c->balance;
-        ctx->set_materialize_grads(false);
-        ctx->mark_non_differentiable({r.idx, r.counts});
-        if (r.loss.defined()) return {r.idx, r.gates, r.counts, r.loss};
-        return {r.idx, r.gates, r.counts};
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list grads)
-    {
-        Tensor dgates = grads[1], dloss = grads.size() > 3 ? grads[3] : Tensor();
-        if (!dgates.defined() && !dloss.defined()) return {Tensor(), Tensor(), Tensor()};
+        std::lock_guard<std::mutex> lock(mutex_);
+        Tensor dgates = grads[0], dloss = grads.size() > 1 ? grads[1] : Tensor();
+        if (!task_should_compute_output(0) || (!dgates.defined() && !dloss.defined())) return {Tensor()};
         const bool again = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
-        const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &valid = saved[1], &idx = saved[2], &counts = saved[3];
+        const Tensor l = x.unpack(), v = valid.unpack(), i = idx.unpack(), n = counts.unpack();
         if (dgates.defined()) dgates = dgates.contiguous();
-        Tensor dx = at::empty({x.size(0), x.size(1)}, x.options().requires_grad(false));
-        const int rc = ((RouteBackwardFn)(uintptr_t)ctx->saved_data["entry"].toInt())(
-            x.data_ptr(), TypeCode(x.scalar_type()), Pitch(x, 0), (int)x.size(0), (int)x.size(1), (int)idx.size(1), (int)ctx->saved_data["scoring"].toInt(),
-            (int)ctx->saved_data["renormalize"].toInt(), (float)ctx->saved_data["scale"].toDouble(), valid.defined() ? (const uint8_t *)valid.data_ptr() : nullptr,
-            (const int32_t *)idx.data_ptr(), dgates.defined() ? (const float *)dgates.data_ptr() : nullptr, (const int32_t *)counts.data_ptr(), (float)ctx->saved_data["balance"].toDouble(),
-            dloss.defined() ? (const float *)dloss.data_ptr() : nullptr, dx.data_ptr(), x.size(1), StreamOf(x.get_device()));
+        Tensor dx = at::empty({l.size(0), l.size(1)}, l.options().requires_grad(false));
+        const int rc = backward(l.data_ptr(), TypeCode(l.scalar_type()), Pitch(l, 0), (int)l.size(0), (int)l.size(1), topk, scoring, renormalize, scale,
+                                v.defined() ? (const uint8_t *)v.data_ptr() : nullptr, (const int32_t *)i.data_ptr(), dgates.defined() ? (const float *)dgates.data_ptr() : nullptr,
+                                (const int32_t *)n.data_ptr(), balance, dloss.defined() ? (const float *)dloss.data_ptr() : nullptr, dx.data_ptr(), l.size(1), StreamOf(l.get_device()));
         TORCH_CHECK(rc == 0, "HcommMoeRouteBackward failed with ", rc);
         if (again) {        // a gradient of the gradient is not offered: asking for it is an error, not a silent zero
             dx.set_requires_grad(true);
             auto error = std::make_shared<torch::autograd::DelayedError>("route: the backward pass is not differentiable", 1);
             dx = (*error)({dx})[0];
         }
-        return {dx, Tensor(), Tensor()};
+        return {dx};
     }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data(); valid.reset_data(); idx.reset_data(); counts.reset_data();
+    }
+    std::string name() const override { return "RouteBackward"; }
 };
+Routed ForwardWithGraph(const RouteCall &c, const Tensor &x)
+{
+    Routed r;
+    {
+        at::AutoGradMode off(false);
+        r = Forward(c, x);
+    }
+    if (r.rc) return r;
+    std::shared_ptr<RouteNode> node(new RouteNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->x = SavedVariable(x, false);
+    node->valid = SavedVariable(c.valid ? *c.valid : Tensor(), false);
+    node->idx = SavedVariable(r.idx, false);
+    node->counts = SavedVariable(r.counts, false);
+    node->backward = c.backward;
+    node->topk = c.topk; node->scoring = c.scoring; node->renormalize = c.renormalize;
+    node->scale = c.scale; node->balance = c.balance;
+    torch::autograd::set_history(r.gates, node);
+    if (r.loss.defined()) torch::autograd::set_history(r.loss, node);
+    return r;
+}
 
 // moe_route(entry, backward entry, scratch size entry, logits, topk, scoring, renormalize, scale, bias or None, valid or None, balance)
 // -> (choices, gates, counts with the number of tokens behind them, loss or None), an error code, or None
@@ -262,15 +280,9 @@ PyObject *Route(PyObject *, PyObject *const *args, Py_ssize_t n)
     int rc = 0;
     {
         pybind11::gil_scoped_release unlocked;
-        if (x->requires_grad() && at::GradMode::is_enabled()) {
-            variable_list out = RouteNode::apply(*x, (const RouteCall *)&c, &rc);
-            idx = out[0]; gates = out[1]; counts = out[2];
-            if (out.size() > 3) loss = out[3];
-        } else {
-            Routed r = Forward(c, *x);
-            idx = r.idx; gates = r.gates; counts = r.counts; loss = r.loss;
-            rc = r.rc;
-        }
+        Routed r = x->requires_grad() && at::GradMode::is_enabled() ? ForwardWithGraph(c, *x) : Forward(c, *x);
+        idx = std::move(r.idx); gates = std::move(r.gates); counts = std::move(r.counts); loss = std::move(r.loss);
+        rc = r.rc;
         if (!rc) counts = counts.narrow(0, 0, e);
     }
     if (rc) return PyLong_FromLong(rc);

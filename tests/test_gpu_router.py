@@ -154,6 +154,18 @@ def test_gradients_of_one_output_alone():
     (a,) = torch.autograd.grad(r.gates.sum(), x, retain_graph=True)
     (b,) = torch.autograd.grad(r.gates, x, torch.ones_like(r.gates))
     assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(r.gates.sum(), x)
+    # logits that are themselves the result of something, used twice, changed in between
+    y = x * 2
+    a, c = route(y, 6, balance=BALANCE), route(y, 3)
+    (d,) = torch.autograd.grad(a.gates.sum() + a.loss + c.gates.sum(), x)
+    (e,), (f,) = (torch.autograd.grad(v, y) for v in (route(y, 6, balance=BALANCE).loss, route(y, 3, balance=BALANCE).gates.square().sum()))
+    assert torch.isfinite(d).all() and torch.allclose(d, 2 * e, rtol=1e-4, atol=1e-6) and f.abs().sum() > 0       # gates of a token add up to 1
+    r = route(y, 6)
+    y.detach().mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(r.gates.sum(), x)
     with torch.no_grad():
         assert not route(x, 6, balance=BALANCE).gates.requires_grad
     assert not r.topk_idx.requires_grad and not r.counts.requires_grad

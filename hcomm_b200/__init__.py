@@ -2,7 +2,7 @@
 
 Layout
     hcomm_b200.comm      Communicator (ctypes over libhcomm.so), group calls
-    hcomm_b200.ops       fused compute + collective operators and their unfused baselines
+    hcomm_b200.ops       fused compute + collective operators and their unfused baselines, routing, 4-bit quantisation and products
     hcomm_b200.parallel  tensor / expert / data parallel building blocks, torch ProcessGroup backend
     hcomm_b200.models    reference model definitions used by the benchmarks
     hcomm_b200.utils     launch helpers, tuning, timing

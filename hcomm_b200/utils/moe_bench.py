@@ -8,7 +8,8 @@ the owners' memory over NVLink) and ONE combine kernel (rows pushed home, gate-w
 Baseline: the same data movement with separate kernels and NCCL: quantise (PyTorch ops), sort rows by destination,
 all_to_all_single of the counts, of the fp8 rows and of the scales; combine = all_to_all_single of the bf16 rows
 back, un-sort, weighted sum.  Router logits are N(0,1); the top-k experts of a token are the largest logits, the
-gates their softmax.  Times are CUDA-event medians with an L2 flush between iterations, maximum over ranks.
+gates their softmax.  With ``--intermediate F`` the whole layer as well: router, routing, exchange and the experts' gated
+feed-forward of that width in 4 bits (``parallel.ep.ExpertParallelMlp``), bytes of its weights and arithmetic per second on this rank.  Times are CUDA-event medians with an L2 flush between iterations, maximum over ranks.
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ from .launch import env_rank
 from .timing import time_cuda
 from ..comm import Communicator, get_root_info
 from ..ops.moe import MoeExchange, quantize_e4m3_1x128
+from ..parallel.ep import ExpertParallelMlp
 
 
 def main():
@@ -30,6 +32,7 @@ def main():
     ap.add_argument("--topk", type=int, default=8)
     ap.add_argument("--hidden", type=int, default=7168)
     ap.add_argument("--tokens", type=int, default=4096)
+    ap.add_argument("--intermediate", type=int, default=0)
     ap.add_argument("--iters", type=int, default=8)
     ap.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args()
@@ -110,10 +113,16 @@ def main():
     bd_ms, _ = time_cuda(lambda: base_dispatch(), a.iters, a.warmup, True, barrier)
     bc_ms, _ = time_cuda(lambda: base_combine(), a.iters, a.warmup, True, barrier)
 
-    t = torch.tensor([d_ms, c_ms, bd_ms, bc_ms], device=dev, dtype=torch.float64)
+    l_ms = 0.0
+    if a.intermediate:
+        layer = ExpertParallelMlp(comm, E, K, H, a.intermediate, T)
+        l_ms, _ = time_cuda(lambda: layer(x), a.iters, a.warmup, True, barrier)
+        layer.destroy()
+
+    t = torch.tensor([d_ms, c_ms, bd_ms, bc_ms, l_ms], device=dev, dtype=torch.float64)
     if world > 1:
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
-    d_ms, c_ms, bd_ms, bc_ms = t.tolist()
+    d_ms, c_ms, bd_ms, bc_ms, l_ms = t.tolist()
     if rank == 0:
         remote = (world - 1) / world
         disp_bytes = T * K * (H + H // 128 * 4 + 8) * remote        # fp8 rows + scales + origin leaving a GPU
@@ -125,6 +134,8 @@ def main():
                           "speedup_dispatch": round(bd_ms / d_ms, 2), "speedup_combine": round(bc_ms / c_ms, 2),
                           "dispatch_frac_of_link_roofline": round(disp_bytes / link / (d_ms * 1e-3), 3) if world > 1 else None,
                           "combine_frac_of_link_roofline": round(comb_bytes / link / (c_ms * 1e-3), 3) if world > 1 else None,
+                          **({"intermediate": a.intermediate, "layer_us": round(l_ms * 1e3, 1), "layer_tflops": round(6e-9 * T * K * H * a.intermediate / l_ms, 1),
+                              "layer_weight_gb": round(epr * 3 * H * a.intermediate * 17 / 32 / 1e9, 2)} if a.intermediate else {}),
                           "max_err": err}), flush=True)
     torch.cuda.synchronize()
     moe.destroy()

@@ -110,7 +110,7 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 // 2048 x 4096 x 1024 15.6 / 10.4, 4096 x 4096 x 4096 37.5 / 29.1, 8192 x 28672 x 8192 880 / 646; 32 experts, 7168 and 2048, gated and down: 64 rows
 // 66 / 81 and 37 / 53, 3000 95 / 112 and 60 / 67, 8000 142 / 140 and 107 / 89, 16000 237 / 225 and 180 / 144.
 //
-// Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles fit at once and that is estimated to be
+// Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles that there can be fit at once and that is estimated to be
 // faster: exchanging sums takes 0.9 us, 0.2 a CTA and 12 ns a row.  us, alone / 2 / 4 / 8 of them: 1 x 4096 x 14336 15.0 / 10.6 / 9.5 / -,
 // 16 x 8192 x 28672 28.1 / 24.7 / - / -, 128 x 1024 x 4096 8.4 / 8.5 / 7.0 / 7.1, 16 x 8192 x 3584 6.8 / 7.6 / - / -, 16 x 4096 x 1024 3.8 / 4.5 / 5.2 / -.
 struct Costs { double single, pair; int split; };
@@ -127,9 +127,10 @@ Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, 
     Costs c = {std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 2.8 * used / 128), pair, 1};
     c.single = 3.0 + std::max(c.single, hbm) + 0.5;
     c.pair = 3.0 + std::max(c.pair, hbm) + 0.5;
-    for (int i = 0; i < 3 && experts == 0; ++i) {
+    const double most = (double)(experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128) * std::ceil(N / 128.0);
+    for (int i = 0; i < 3; ++i) {
         const int split = 2 << i;
-        if (tiles(128, 128) > clusters[i] || stages < split) continue;
+        if (most > clusters[i] || stages < split) continue;
         const double us = 3.0 + std::max(std::ceil(stages / split) * stage, hbm) + 0.9 + 0.2 * split + 0.012 * used;
         if (us < c.single) { c.single = us; c.split = split; }
     }

@@ -39,7 +39,8 @@ def test_ctas_that_share_a_tile(shape, splits):
 
 def test_nothing_is_shared_where_clusters_do_not_fit():
     assert ask(1, 4096, 14336, clusters=(31, 0, 0))[0] == 1 and ask(1, 4096, 14336, clusters=(32, 0, 0))[0] == 2
-    assert ask(8, 7168, 2048, 32)[0] == 1           # how many tiles there are is known on the device only
+    # by expert: as many tiles as any split of the rows makes
+    assert ask(8, 7168, 2048, 32)[0] == 1 and ask(1, 4096, 14336, 8)[0] == 4 and ask(2, 4096, 14336, 8)[0] == 2 and ask(2, 4096, 14336, 8, clusters=(63, 33, 15))[0] == 1
     assert ask(1, 128, 512)[0] <= 2                 # never more CTAs than stages
 
 

@@ -308,6 +308,12 @@ def test_tiles_that_ctas_share_along_k(m, n, k, gated):
     assert torch.equal(big[:, 1:n + 1], outs[0]) and not big[:, 0].any() and not big[:, n + 1:].any()
 
 
+@pytest.mark.parametrize("rows,n,k,split", [(8, 1024, 4096, [0, 1, 1, 3, 8]), (40, 500, 2080, [0, 0, 40]), (6, 256, 8192, [2, 2, 2, 2]), (130, 130, 1024, [0, 129, 130, 130]), (3, 1000, 768, [0] + [1] * 40)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_tiles_of_experts_that_ctas_share_along_k(rows, n, k, split, gated):
+    test_products_by_expert(rows, n, k, split, gated)
+
+
 def test_refusals():
     from hcomm_b200.ops.fp4 import Fp4Tensor, dequantize_fp4, gemm_fp4, gemm_fp4_swiglu, quantize_fp4
     torch.cuda.set_device(0)

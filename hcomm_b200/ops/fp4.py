@@ -9,7 +9,7 @@
 
 A value is e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives); every 32 consecutive ones of a row share a power of two, the
 largest that keeps the block's largest magnitude at 4 or more before rounding (at least 2^-127).  Rounding is to the nearest, the even
-one of two; magnitudes beyond 6 become 6.  A block that holds an infinity or a NaN becomes NaN.
+one of two; magnitudes beyond 6 become 6.  A block that holds an infinity or a NaN becomes NaN.  None of these operators has a gradient.
 """
 from __future__ import annotations
 

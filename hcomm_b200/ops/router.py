@@ -13,6 +13,7 @@ tokens' choices that went to expert e and P_e the tokens' mean probability of it
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -33,9 +34,13 @@ class _ShortRoute(Short):
 
     __slots__ = ("_others",)
 
+    def find(self):
+        self._others = entry("HcommMoeRouteBackward"), entry("HcommMoeRouteScratchBytes")      # before another thread can see the call
+        return super().find()
+
     def __call__(self, *args):
-        if self._call is None and self.find() is not None:
-            self._others = entry("HcommMoeRouteBackward"), entry("HcommMoeRouteScratchBytes")
+        if self._call is None:
+            self.find()
         return super().__call__(*self._others, *args)
 
 
@@ -147,6 +152,7 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", renormal
     if logits.dim() != 2 or logits.dtype not in _TYPES:
         raise TypeError("logits must be [T, experts] in fp32, fp16 or bf16")
     t, e = logits.shape
+    topk = operator.index(topk)
     if not 1 <= e <= MAX_EXPERTS or not 1 <= topk <= min(e, MAX_TOPK):
         raise ValueError(f"{topk} of {e} experts: at least one and at most {MAX_TOPK} of at most {MAX_EXPERTS}")
     if not logits.is_cuda:

@@ -50,7 +50,11 @@ class ExpertParallelMlp:
         self._y = torch.zeros((rows, hidden), dtype=torch.bfloat16, device=dev)
 
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, valid: torch.Tensor | None = None) -> torch.Tensor:
-        """x [tokens, hidden] bf16; tokens that ``valid`` (bool [tokens]) takes out go to no expert and come back as 0."""
+        """x [tokens, hidden] bf16; tokens that ``valid`` (bool [tokens]) takes out go to no expert and come back as 0.  A rank without
+        tokens takes part all the same, as the pass is collective: with one that is taken out."""
+        if x.shape[0] == 0:
+            self.forward(x.new_zeros((1, x.shape[1])), valid=torch.zeros(1, dtype=torch.bool, device=x.device))
+            return torch.empty_like(x) if out is None else out
         r = self.routing = route(gemm_bf16(x, self.router), self.topk, valid=valid, **self.options)
         recv = self.moe.dispatch(x, r.topk_idx)
         offsets = recv.expert_offsets

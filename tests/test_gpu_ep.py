@@ -72,6 +72,23 @@ def test_each_step_of_one_rank(tokens, experts, topk, hidden, inter, scoring):
         end(comms, [layer])
 
 
+def test_batches_of_every_size_and_none():
+    g = gen(5)
+    comms, (layer,) = make(1, experts=16, topk=4, hidden=512, intermediate=96, max_tokens=200)
+    try:
+        x = torch.randn(200, 512, device="cuda", generator=g).to(torch.bfloat16)
+        whole = layer(x).clone()
+        for n in (200, 1, 33, 0, 128, 2):
+            assert torch.equal(layer(x[:n]), whole[:n])
+            assert int(layer.routing.counts.sum()) == 4 * n
+        assert not layer(x, valid=torch.zeros(200, dtype=torch.bool, device="cuda")).any()
+        assert layer.moe.overflow() == 0
+        with pytest.raises(Exception):
+            layer(torch.cat([x, x]))
+    finally:
+        end(comms, [layer])
+
+
 def test_two_ranks_give_what_one_gives():
     from hcomm_b200.ops.fp4 import Fp4Tensor, quantize_fp4
     g = gen(77)
@@ -107,6 +124,9 @@ def test_two_ranks_give_what_one_gives():
     for _ in range(2):
         outs = run_ranks(2, step)
         assert torch.equal(torch.cat(outs), want)
+    xs[1] = xs[1][:0]           # a rank without tokens; the other's go to the experts of both
+    outs = run_ranks(2, step)
+    assert torch.equal(outs[0], want[:tokens]) and outs[1].shape == (0, hidden)
     assert all(x.moe.overflow() == 0 for x in layers)
     end(comms, layers)
 

@@ -344,6 +344,8 @@ def test_refusals():
     with pytest.raises(ValueError):
         gemm_fp4_swiglu(q, b, quantize_fp4(torch.zeros(32, 128, device="cuda")))
     assert gemm_fp4(quantize_fp4(x[:0]), b).shape == (0, 16)
+    none = quantize_fp4(x[:0], offsets=torch.zeros(3, device="cuda", dtype=torch.int32))
+    assert gemm_fp4(none, w).shape == (0, 16) and dequantize_fp4(none).shape == (0, 128)
     with pytest.raises(ValueError):
         gemm_fp4(quantize_fp4(x[:, :0]), quantize_fp4(torch.zeros(16, 0, device="cuda")))
 

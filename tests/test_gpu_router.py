@@ -324,10 +324,40 @@ def test_sums_over_a_communicator():
         comm.destroy()
 
 
+def test_threads_whose_calls_are_the_first():
+    import subprocess
+    import sys
+    from pathlib import Path
+    program = """
+import sys, threading
+sys.path.insert(0, {root!r})
+import torch
+from hcomm_b200.ops.router import route
+x = torch.randn(40, 64, device="cuda")
+got, bad = [], []
+def work():
+    try:
+        got.append(route(x, 4).topk_idx)
+    except BaseException as e:
+        bad.append(e)
+threads = [threading.Thread(target=work) for _ in range(16)]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+print(len(got), bad, all(torch.equal(g, got[0]) for g in got))
+""".format(root=str(Path(__file__).resolve().parent.parent))
+    res = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and res.stdout.split() == ["16", "[]", "True"], res.stdout + res.stderr
+
+
 def test_refusals():
+    import numpy as np
     from hcomm_b200.ops.router import route
     torch.cuda.set_device(0)
     x = torch.zeros(4, 8, device="cuda")
+    assert torch.equal(route(x, np.int64(3)).topk_idx, route(x, 3).topk_idx)
+    with pytest.raises(TypeError):
+        route(x, 2.0)
     for error, args, kw in ((ValueError, (x, 9), {}), (ValueError, (x, 0), {}), (ValueError, (x, 2), dict(scoring="tanh")), (TypeError, (x.long(), 2), {}), (TypeError, (x[0], 2), {}),
                             (ValueError, (x.t(), 2), {}), (ValueError, (x.cpu(), 2), {}), (ValueError, (torch.zeros(2, 1025, device="cuda"), 2), {}),
                             (ValueError, (torch.zeros(2, 64, device="cuda"), 17), {}), (ValueError, (x, 2), dict(bias=torch.zeros(8, device="cuda"))),

@@ -350,6 +350,14 @@ def test_refusals():
         gemm_fp4(quantize_fp4(x[:, :0]), quantize_fp4(torch.zeros(16, 0, device="cuda")))
 
 
+def test_rows_wider_than_a_grid():
+    from hcomm_b200.ops.fp4 import dequantize_fp4, quantize_fp4
+    x = torch.randn(2, 32 * 200001, device="cuda", generator=gen(52)).to(torch.bfloat16)
+    back = dequantize_fp4(quantize_fp4(x))
+    for at in range(0, x.shape[1], 320000):
+        assert same(back[:, at:at + 320000], nearest(x[:, at:at + 320000]))
+
+
 def test_a_checkpoint_that_is_not_aligned():
     from hcomm_b200.ops.fp4 import Fp4Tensor, gemm_fp4, quantize_fp4
     g = gen(51)

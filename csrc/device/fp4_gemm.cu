@@ -169,7 +169,7 @@ HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, vo
     const bool pairs = dev.pairs > 0 && M > 128 && costs.pair < costs.single;
     g.tilesN = pairs && !glu ? (N + 255) / 256 : (N + 127) / 128;
     g.group = pairs ? 8 : 16;
-    if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX || rowTiles * g.tileCols > INT32_MAX) {
+    if (rowTiles * g.tilesN > INT32_MAX / 2 || (int64_t)matrices * g.tileRowsB * g.tileCols > INT32_MAX / 2 || rowTiles * g.tileCols > INT32_MAX / 2) {
         RPT_ERR("EI0003", "%s: %d x %d x %d is more than a launch can count", what, M, N, K);
         return HCCL_E_PARA;
     }

@@ -102,13 +102,13 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 // 128 columns): the less of two estimates, in us.
 //   * tiles come in waves of what fits at once; of grouped rows, which are known on the device only, every expert is taken to have the
 //     average, and a tile that it fills half;
-//   * single: a stage of 256 columns of K takes 0.19 us to issue, or its bytes at 112 a ns; a tile at least 0.4 us and 2.8 a 128 rows, in which
+//   * single: a stage of 256 columns of K takes 0.19 us to issue, or its bytes at 112 a ns; a tile at least 0.4 us and 1.6 a 128 rows, in which
 //     the tile in front is stored;
 //   * pair: 0.34 us a stage, and 1.5 in which nothing overlaps the reading of the tile's accumulator;
 //   * nothing is faster than its bytes at 6.5 TB/s.
 // us, single / pair: 500 x 3584 x 8192 13.7 / 15.1, 777 x 3584 x 8192 21.5 / 16.0, 256 x 8192 x 28672 34.8 / 41.1, 1024 x 1024 x 4096 9.0 / 10.0,
-// 2048 x 4096 x 1024 15.6 / 10.4, 4096 x 4096 x 4096 37.5 / 29.1, 8192 x 28672 x 8192 880 / 646; 32 experts, 7168 and 2048, gated and down: 64 rows
-// 66 / 81 and 37 / 53, 3000 95 / 112 and 60 / 67, 8000 142 / 140 and 107 / 89, 16000 237 / 225 and 180 / 144.
+// 2048 x 4096 x 1024 11.5 / 10.5, 4096 x 4096 x 4096 36 / 29, 8192 x 28672 x 8192 862 / 642; 32 experts, 7168 and 2048, gated and down: 64 rows
+// 67 / 81 and 37 / 54, 3000 94 / 111 and 55 / 66, 5003 106 / 123 and 69 / 76, 8000 138 / 137 and 91 / 88, 16000 234 / 215 and 153 / 142.
 //
 // Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles that there can be fit at once and that is estimated to be
 // faster: exchanging sums takes 0.9 us, 0.2 a CTA and 12 ns a row.  us, alone / 2 / 4 / 8 of them: 1 x 4096 x 14336 15.0 / 10.6 / 9.5 / -,
@@ -124,7 +124,7 @@ Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, 
     const double hbm = (17.0 / 32 * (M * K + matrices * (glu ? 2 : 1) * N * K) + 2.0 * M * N) / 6.5e6;
     const double used = std::min(rows, 128.0), stage = std::max(0.19, ((glu ? 2 : 1) * 17408 + 1024 + 128 * used) / 112e3);
     const double pair = std::ceil(tiles(256, glu ? 128 : 256) / std::max(pairs, 1)) * (stages * 0.34 + 1.5);
-    Costs c = {std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 2.8 * used / 128), pair, 1};
+    Costs c = {std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 1.6 * used / 128), pair, 1};
     c.single = 3.0 + std::max(c.single, hbm) + 0.5;
     c.pair = 3.0 + std::max(c.pair, hbm) + 0.5;
     const double most = (double)(experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128) * std::ceil(N / 128.0);

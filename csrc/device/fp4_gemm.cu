@@ -105,7 +105,7 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 //   * single: a stage of 256 columns of K takes 0.19 us to issue, or its bytes at 112 a ns; a tile at least 0.4 us and 1.6 a 128 rows, in which
 //     the tile in front is stored;
 //   * pair: 0.34 us a stage, and 1.5 in which nothing overlaps the reading of the tile's accumulator;
-//   * nothing is faster than its bytes at 6.5 TB/s.
+//   * nothing is faster than its bytes at 6.5 TB/s, pairs at 4.6: they have less of B under way.
 // us, single / pair: 500 x 3584 x 8192 13.7 / 15.1, 777 x 3584 x 8192 21.5 / 16.0, 256 x 8192 x 28672 34.8 / 41.1, 1024 x 1024 x 4096 9.0 / 10.0,
 // 2048 x 4096 x 1024 11.5 / 10.5, 4096 x 4096 x 4096 36 / 29, 8192 x 28672 x 8192 862 / 642; 32 experts, 7168 and 2048, gated and down: 64 rows
 // 67 / 81 and 37 / 54, 3000 94 / 111 and 55 / 66, 5003 106 / 123 and 69 / 76, 8000 138 / 137 and 91 / 88, 16000 234 / 215 and 153 / 142.
@@ -126,7 +126,7 @@ Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, 
     const double pair = std::ceil(tiles(256, glu ? 128 : 256) / std::max(pairs, 1)) * (stages * 0.34 + 1.5);
     Costs c = {std::ceil(tiles(128, 128) / sms) * std::max(stages * stage, 0.4 + 1.6 * used / 128), pair, 1};
     c.single = 3.0 + std::max(c.single, hbm) + 0.5;
-    c.pair = 3.0 + std::max(c.pair, hbm) + 0.5;
+    c.pair = 3.0 + std::max(c.pair, 1.4 * hbm) + 0.5;
     const double most = (double)(experts > 0 ? GroupedTileRows(M, experts) : (M + 127) / 128) * std::ceil(N / 128.0);
     for (int i = 0; i < 3; ++i) {
         const int split = 2 << i;

@@ -123,7 +123,8 @@ def test_gradient_against_differences(scoring, renormalize):
     t, e, k = 24, 20, 3
     x, _ = make(g, t, e, torch.float32, False)
     dgates = torch.randn(t, k, device="cuda", generator=g)
-    idx, _, counts, tokens, _ = reference(x, k, scoring, renormalize)
+    idx, share, counts, tokens, p = reference(x, k, scoring, renormalize)
+    _, size = gradient(x, idx, share, counts, tokens, p, scoring, renormalize, dgates, torch.tensor(3.0, device="cuda", dtype=torch.float64), k)
 
     def value(x64):
         _, share, _, _, p = reference(x64, k, scoring, renormalize, idx=idx)
@@ -135,8 +136,10 @@ def test_gradient_against_differences(scoring, renormalize):
         v = torch.randn(t, e, device="cuda", generator=g, dtype=torch.float64)
         h = 1e-5
         difference = (value(x.detach().double() + h * v) - value(x.detach().double() - h * v)) / (2 * h)
-        # 480 terms, each off by 2^-18 of magnitudes below 10, and h^2 times the third derivative
-        assert abs((x.grad.double() * v).sum() - difference) < 480 * 10 * 2.0 ** -18 * 0.1
+        # each entry of the gradient is off as in the test above; the difference by h^2 times a third derivative along v, below 10^4 here, and by
+        # 2^-52 of values below 100 divided by h
+        tol = ((3 * relative(x.detach(), e) + 2.0 ** -21 + 2.0 ** -24) * size * v.abs()).sum() + 1e-6 + 1e-8
+        assert abs((x.grad.double() * v).sum() - difference) < tol
 
 
 def test_gradients_of_one_output_alone():

@@ -79,7 +79,7 @@ template <int BN> struct Config {
     static constexpr int kScaleCols = 8 + BN / 128 * 8;             // of a stage, in tensor memory
     static constexpr int kScaleBase = kAccumulators * BN;
     static constexpr int kTail = 256;
-    __host__ __device__ static constexpr int ASlot(int boxRows, bool grouped) { return grouped || boxRows > 64 ? 128 * 128 : boxRows < 8 ? 1024 : boxRows * 128; }
+    __host__ __device__ static constexpr int ASlot(int boxRows, bool grouped) { return (grouped ? 128 : boxRows) * 128; }
     static constexpr int StageBytes(int aSlot) { return aSlot + kBBytes + kSaBytes + kSbBytes; }
     static constexpr int Stages(int aSlot, int experts)
     {

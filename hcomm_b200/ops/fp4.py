@@ -24,6 +24,7 @@ from .._stream import raw_stream
 
 _TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16, torch.float8_e4m3fn: _lib.FP8E4M3}
 MAX_EXPERTS = 1024
+_MOST = 2 ** 31 - 257          # rows, columns and depth of a product, which the library takes as 32-bit numbers
 
 
 _short_quantize, _short_dequantize = Short("fp4_quantize", "HcommFp4Quantize"), Short("fp4_dequantize", "HcommFp4Dequantize")
@@ -201,6 +202,8 @@ def _result(what: str, a: Fp4Tensor, weights, out):
     if shape[-1] == 0:
         raise ValueError("no columns to multiply")
     m, n = a.shape[0], shape[-2]
+    if max(m, n, shape[-1]) > _MOST:
+        raise ValueError(f"a product of {m} x {n} x {shape[-1]}: at most {_MOST} of each")
     if out is None:
         out = torch.empty((m, n), dtype=torch.bfloat16, device=device)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (m, n) or out.device != device:

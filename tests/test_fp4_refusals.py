@@ -101,3 +101,15 @@ def test_host_tensors_and_parts_that_do_not_fit():
     grouped = Fp4Tensor(q.values, q.scales, torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError):
         grouped.block_scales()
+
+
+@pytest.mark.parametrize("m, n", [((1 << 32) + 5, 8), (8, (1 << 32) + 5), ((1 << 31) - 256, 8)])
+def test_products_refuse_more_rows_than_they_count(monkeypatch, m, n):
+    """Sizes go to the library as 32-bit numbers: none may be cut to its lower bits."""
+    from hcomm_b200.ops import fp4
+    monkeypatch.setattr(fp4, "_on_device", lambda what, *tensors: tensors[0].device)
+
+    def operand(rows):
+        return Fp4Tensor(torch.empty((rows, 16), dtype=torch.uint8, device="meta"), torch.empty((_scale_tiles(1, rows, 32, 0), 512), dtype=torch.uint8, device="meta"))
+    with pytest.raises(ValueError, match="at most"):
+        fp4._result("gemm_fp4", operand(m), (operand(n),), None)

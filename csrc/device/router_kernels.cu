@@ -34,6 +34,7 @@
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopk = 16;
+constexpr int kMostTokens = INT32_MAX - 32;      // rounded up to a block's tokens still a 32-bit number
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr int kFinishThreads = 1024, kFinishCtas = 8;
 
@@ -678,7 +679,7 @@ template <bool BACKWARD> HcclResult LaunchTyped(const char *what, const Params &
 int BytesOf(int dataType) { return dataType == HCCL_DATA_TYPE_FP32 ? 4 : 2; }
 HcclResult CheckShape(const char *what, int dataType, int64_t ld, int tokens, int experts, int topk, int scoring, const float *bias)
 {
-    if ((dataType != HCCL_DATA_TYPE_FP32 && dataType != HCCL_DATA_TYPE_FP16 && dataType != HCCL_DATA_TYPE_BFP16) || tokens < 0 || experts < 1 || experts > kMaxExperts || topk < 1 ||
+    if ((dataType != HCCL_DATA_TYPE_FP32 && dataType != HCCL_DATA_TYPE_FP16 && dataType != HCCL_DATA_TYPE_BFP16) || tokens < 0 || tokens > kMostTokens || experts < 1 || experts > kMaxExperts || topk < 1 ||
         topk > kMaxTopk || topk > experts || ld < experts || (scoring != HCOMM_MOE_SOFTMAX && scoring != HCOMM_MOE_SIGMOID) || (bias && scoring != HCOMM_MOE_SIGMOID)) {
         RPT_ERR("EI0003", "%s: type %d (FP32, FP16, BFP16), %d tokens, %d experts (<= %d) %lld apart, %d of them chosen (<= %d), scoring %d%s", what, dataType, tokens, experts, kMaxExperts,
                 (long long)ld, topk, kMaxTopk, scoring, bias ? " with a bias, which only the sigmoid takes" : "");
@@ -696,7 +697,7 @@ bool Vectors(const void *base, int64_t ld, int experts, int dataType)
 
 extern "C" uint64_t HcommMoeRouteScratchBytes(int tokens, int experts)
 {
-    if (tokens < 0 || experts < 1 || experts > kMaxExperts) return 0;
+    if (tokens < 0 || tokens > kMostTokens || experts < 1 || experts > kMaxExperts) return 0;
     const int blocks = BlocksOf(tokens, experts, kMostBlocks);
     return blocks == 1 ? 0 : (uint64_t)blocks * (2 * experts + 1) * 4;
 }

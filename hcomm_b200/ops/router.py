@@ -27,6 +27,7 @@ from ..comm import Communicator
 SCORINGS = {"softmax": 0, "sigmoid": 1}
 _TYPES = {torch.float32: _lib.FP32, torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 MAX_EXPERTS, MAX_TOPK = 1024, 16
+_MOST_TOKENS = 2 ** 31 - 33           # the library counts them in 32 bits
 
 
 class _ShortRoute(Short):
@@ -155,6 +156,8 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", renormal
     topk = operator.index(topk)
     if not 1 <= e <= MAX_EXPERTS or not 1 <= topk <= min(e, MAX_TOPK):
         raise ValueError(f"{topk} of {e} experts: at least one and at most {MAX_TOPK} of at most {MAX_EXPERTS}")
+    if t > _MOST_TOKENS:
+        raise ValueError(f"{t} tokens: at most {_MOST_TOKENS}")
     if not logits.is_cuda:
         raise ValueError(f"expected a tensor on a CUDA device, but got one on {logits.device}")
     if (e > 1 and logits.stride(1) != 1) or (t > 1 and logits.stride(0) < e):

@@ -48,3 +48,11 @@ def test_host_tensors():
     from hcomm_b200.ops.router import route
     with pytest.raises(ValueError, match="CUDA"):
         route(torch.zeros(4, 8), 2)
+
+
+def test_more_tokens_than_are_counted():
+    from hcomm_b200.ops.router import _scratch_bytes, route
+    for tokens in ((1 << 31) - 1, (1 << 31) - 31):
+        assert forward(tokens=tokens) == PARA and backward(tokens=tokens) == PARA and _scratch_bytes(tokens, 8) == 0
+    with pytest.raises(ValueError, match="tokens"):
+        route(torch.empty((1 << 32) + 4, 8, device="meta"), 2)

@@ -263,11 +263,13 @@ PyObject *Route(PyObject *, PyObject *const *args, Py_ssize_t n)
     if (!x || x->dim() != 2 || (x->scalar_type() != at::kFloat && x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
     void *f, *b, *s;
     if (!Address(args[0], &f) || !Address(args[1], &b) || !Address(args[2], &s)) Py_RETURN_NONE;
-    RouteCall c{(RouteFn)f, (RouteBackwardFn)b, (ScratchFn)s, (int)PyLong_AsLong(args[4]), (int)PyLong_AsLong(args[5]), (int)PyLong_AsLong(args[6]),
+    const long topk = PyLong_AsLong(args[4]);           // whole: 2^32 + 2 is not 2
+    if (topk < 1 || topk > 16) { PyErr_Clear(); Py_RETURN_NONE; }
+    RouteCall c{(RouteFn)f, (RouteBackwardFn)b, (ScratchFn)s, (int)topk, (int)PyLong_AsLong(args[5]), (int)PyLong_AsLong(args[6]),
                 (float)PyFloat_AsDouble(args[7]), (float)PyFloat_AsDouble(args[10]), nullptr, nullptr};
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
     const int64_t t = x->size(0), e = x->size(1);
-    if (t < 1 || t > INT32_MAX || e < 1 || e > 1024 || c.topk < 1 || c.topk > 16 || c.topk > e || (e > 1 && x->stride(1) != 1) || (t > 1 && x->stride(0) < e)) Py_RETURN_NONE;
+    if (t < 1 || t > INT32_MAX || e < 1 || e > 1024 || topk > e || (e > 1 && x->stride(1) != 1) || (t > 1 && x->stride(0) < e)) Py_RETURN_NONE;
     if (args[8] != Py_None) {
         c.bias = Plain(args[8], dev);
         if (!c.bias || c.scoring != 1 || c.bias->scalar_type() != at::kFloat || c.bias->dim() != 1 || c.bias->size(0) != e || !c.bias->is_contiguous()) Py_RETURN_NONE;

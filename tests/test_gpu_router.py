@@ -369,3 +369,10 @@ def test_refusals():
                             (ValueError, (torch.zeros(1, 8, device="cuda").expand(4, 8), 2), {}), (TypeError, (x.double(), 2), {})):
         with pytest.raises(error):
             route(*args, **kw)
+
+
+@pytest.mark.parametrize("topk", [2 ** 32 + 2, 2 ** 64 + 2, -2 ** 32 + 2])
+def test_choices_beyond_32_bits_are_refused(topk):
+    from hcomm_b200.ops.router import route
+    with pytest.raises(ValueError):
+        route(torch.zeros(4, 8, device="cuda"), topk)

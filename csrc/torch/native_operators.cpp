@@ -174,6 +174,7 @@ struct RouteCall {
     ScratchFn scratch;
     int topk, scoring, renormalize;
     float scale, balance;
+    bool lossWanted;            // balance as it was given is not 0, though as a float it may be
     const Tensor *bias, *valid;
 };
 struct Routed {
@@ -185,7 +186,7 @@ Routed Forward(const RouteCall &c, const Tensor &x)
     const int64_t t = x.size(0), e = x.size(1);
     const auto ints = x.options().dtype(at::kInt).requires_grad(false), floats = x.options().dtype(at::kFloat).requires_grad(false);
     Routed r{at::empty({t, c.topk}, ints), at::empty({t, c.topk}, floats), at::empty({e + 1}, ints), Tensor(), 0};
-    if (c.balance != 0) r.loss = at::empty({}, floats);
+    if (c.lossWanted) r.loss = at::empty({}, floats);
     const int64_t bytes = (int64_t)c.scratch((int)t, (int)e);
     Tensor scratch;
     if (bytes) scratch = at::empty({bytes / 4}, ints);
@@ -266,7 +267,7 @@ PyObject *Route(PyObject *, PyObject *const *args, Py_ssize_t n)
     const long topk = PyLong_AsLong(args[4]);           // whole: 2^32 + 2 is not 2
     if (topk < 1 || topk > 16) { PyErr_Clear(); Py_RETURN_NONE; }
     RouteCall c{(RouteFn)f, (RouteBackwardFn)b, (ScratchFn)s, (int)topk, (int)PyLong_AsLong(args[5]), (int)PyLong_AsLong(args[6]),
-                (float)PyFloat_AsDouble(args[7]), (float)PyFloat_AsDouble(args[10]), nullptr, nullptr};
+                (float)PyFloat_AsDouble(args[7]), (float)PyFloat_AsDouble(args[10]), PyFloat_AsDouble(args[10]) != 0, nullptr, nullptr};
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
     const int64_t t = x->size(0), e = x->size(1);
     if (t < 1 || t > INT32_MAX || e < 1 || e > 1024 || topk > e || (e > 1 && x->stride(1) != 1) || (t > 1 && x->stride(0) < e)) Py_RETURN_NONE;

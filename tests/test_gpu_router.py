@@ -5,6 +5,8 @@ it (twice with a log-sigmoid, which is off by four roundings more), exp by 2^-23
 reciprocal and the products by 2^-24; `relative` adds these up.  Sums over tokens have positive terms, so their relative error is that of a
 term plus a rounding for each addition in a row.  A gradient is a difference of such products: the bound is the relative
 error of its terms times their magnitudes, three roundings more, and the rounding to its type."""
+import contextlib
+
 import pytest
 import torch
 
@@ -376,3 +378,13 @@ def test_choices_beyond_32_bits_are_refused(topk):
     from hcomm_b200.ops.router import route
     with pytest.raises(ValueError):
         route(torch.zeros(4, 8, device="cuda"), topk)
+
+
+def test_a_coefficient_that_is_0_in_32_bits_makes_a_loss_of_0():
+    from hcomm_b200.ops.router import route
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    for mode in (contextlib.nullcontext(), torch.overrides.BaseTorchFunctionMode()):        # the native call, and the general one
+        with mode:
+            loss = route(x, 2, balance=1e-50).loss
+        assert loss is not None and loss.item() == 0
+        assert torch.equal(torch.autograd.grad(loss, x)[0], torch.zeros_like(x))

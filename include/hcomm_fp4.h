@@ -46,7 +46,7 @@ int HcommFp4Dequantize(const void *values, const void *scales, int64_t batch, in
 int HcommFp4Gemm(const void *aValues, const void *aScales, const void *bValues, const void *bScales, void *out, int M, int N, int K, int64_t ldOut,
                  const int32_t *offsets, int experts, void *stream);
 /* out[M][N] = silu(A * G^T) * (A * U^T): the gate and up projections of a gated feed-forward layer in one pass over A, the
- * product taken from the fp32 accumulators. */
+ * product taken from the fp32 accumulators.  silu is taken as 0 where its argument is below -87.3 (magnitudes below 2^-119). */
 int HcommFp4GemmSwiglu(const void *aValues, const void *aScales, const void *gValues, const void *gScales, const void *uValues, const void *uScales, void *out,
                        int M, int N, int K, int64_t ldOut, const int32_t *offsets, int experts, void *stream);
 /* Reads and clears the "a bounded wait expired inside a product" flag of the current device (0 = none). */

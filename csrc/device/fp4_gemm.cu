@@ -74,7 +74,7 @@ bool CurrentDevice(Device *d)
 }
 
 struct Operand { const void *values, *scales; };
-constexpr int kMost = INT32_MAX - 256;         // rows and columns: rounded up to a tile still a 32-bit number
+constexpr int kMost = INT32_MAX - 256;         // rows, columns and depth: rounded up to a tile or a stage still a 32-bit number
 
 // boxRows rows x 256 columns of values; `matrices` of them one behind the other.
 HcclResult ValueMap(CUtensorMap *m, const void *values, int64_t matrices, int64_t rows, int64_t K, int boxRows)
@@ -140,9 +140,9 @@ Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, 
 // b[1] is the up projection of a gated product, else NULL.
 HcclResult Gemm(const char *what, Operand a, const Operand (&b)[2], bool glu, void *out, int M, int N, int K, int64_t ldOut, const int32_t *offsets, int experts, void *stream)
 {
-    if (M < 0 || N < 0 || K < 0 || M > kMost || N > kMost || K % kBlock || ldOut < N || experts < 0 || experts > kMaxExperts || (experts > 0) != (offsets != nullptr)) {
-        RPT_ERR("EI0003", "%s: M %d, N %d, K %d (a multiple of %d), rows of the result %lld apart, %d experts (at most %d, with offsets)", what, M, N, K, kBlock, (long long)ldOut,
-                experts, kMaxExperts);
+    if (M < 0 || N < 0 || K < 0 || M > kMost || N > kMost || K > kMost || K % kBlock || ldOut < N || experts < 0 || experts > kMaxExperts || (experts > 0) != (offsets != nullptr)) {
+        RPT_ERR("EI0003", "%s: M %d, N %d, K %d (a multiple of %d; at most %d each), rows of the result %lld apart, %d experts (at most %d, with offsets)", what, M, N, K, kBlock, kMost,
+                (long long)ldOut, experts, kMaxExperts);
         return HCCL_E_PARA;
     }
     if (M == 0 || N == 0) return HCCL_SUCCESS;

@@ -146,7 +146,8 @@ PyObject *Gemm(PyObject *, PyObject *const *args, Py_ssize_t n)
     const int64_t dims = experts ? 3 : 2;
     if (a.values->dim() != 2 || b.values->dim() != dims || b.cols != a.cols || (experts && b.batch != experts) || (gated && u.values->sizes() != b.values->sizes())) Py_RETURN_NONE;
     const int64_t m = a.rows, w = b.rows, k = a.cols;
-    if (m == 0 || w == 0 || k == 0) Py_RETURN_NONE;
+    constexpr int64_t kMost = INT32_MAX - 256;          // of a product, as the entry points have it
+    if (m == 0 || w == 0 || k == 0 || m > kMost || w > kMost || k > kMost) Py_RETURN_NONE;
     Tensor made;
     const Tensor *out = &made;
     if (args[4] == Py_None) made = at::empty({m, w}, a.values->options().dtype(at::kBFloat16).requires_grad(false));

@@ -42,7 +42,7 @@ int HcommFp4Dequantize(const void *values, const void *scales, int64_t batch, in
 
 /* out[M][N] (bf16) = A[M][K] * B[N][K]^T, accumulated in fp32.  With experts > 0 the rows of A are grouped as above and B holds `experts`
  * matrices: rows of expert e are multiplied with matrix e; rows of out behind the last expert's are left as they were.
- * K a multiple of 32; M and N any; rows of out ldOut elements apart.  out may not overlap an operand. */
+ * K a multiple of 32; M, N and K at most 2^31 - 257; rows of out ldOut elements apart.  out may not overlap an operand. */
 int HcommFp4Gemm(const void *aValues, const void *aScales, const void *bValues, const void *bScales, void *out, int M, int N, int K, int64_t ldOut,
                  const int32_t *offsets, int experts, void *stream);
 /* out[M][N] = silu(A * G^T) * (A * U^T): the gate and up projections of a gated feed-forward layer in one pass over A, the

@@ -113,3 +113,11 @@ def test_products_refuse_more_rows_than_they_count(monkeypatch, m, n):
         return Fp4Tensor(torch.empty((rows, 16), dtype=torch.uint8, device="meta"), torch.empty((_scale_tiles(1, rows, 32, 0), 512), dtype=torch.uint8, device="meta"))
     with pytest.raises(ValueError, match="at most"):
         fp4._result("gemm_fp4", operand(m), (operand(n),), None)
+
+
+@pytest.mark.parametrize("k", [(1 << 31) - 256, (1 << 31) - 224, (1 << 31) - 128, (1 << 31) - 32])
+@pytest.mark.parametrize("gated", [False, True])
+def test_products_refuse_a_depth_that_32_bits_cannot_round_up(k, gated):
+    p = ctypes.c_void_p
+    fn = _lib.load().HcommFp4GemmSwiglu if gated else _lib.load().HcommFp4Gemm
+    assert fn(*[p(64)] * (6 if gated else 4), p(64), 1, 1, k, i64(1), p(0), 0, p(0)) == PARA

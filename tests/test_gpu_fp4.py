@@ -418,3 +418,17 @@ def test_threads_and_streams_at_the_same_time():
     for t in threads:
         t.join()
     assert not bad and take_kernel_error() == 0
+
+
+def test_depths_beyond_32_bits_are_refused_by_every_way():
+    import contextlib
+    from hcomm_b200.ops.fp4 import Fp4Tensor, gemm_fp4, gemm_fp4_swiglu
+    torch.cuda.set_device(0)
+    k = 2 ** 31 - 128
+    q = Fp4Tensor(torch.empty(1, k // 2, device="cuda", dtype=torch.uint8), torch.empty(k // 128, 512, device="cuda", dtype=torch.uint8))         # 10 GB
+    for mode in (contextlib.nullcontext(), torch.overrides.BaseTorchFunctionMode()):        # the native call, and the general one
+        with mode:
+            with pytest.raises(ValueError, match="at most"):
+                gemm_fp4(q, q)
+            with pytest.raises(ValueError, match="at most"):
+                gemm_fp4_swiglu(q, q, q)

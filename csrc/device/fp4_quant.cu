@@ -45,14 +45,20 @@ __device__ __forceinline__ Range RowsOf(const Rows &r, int *start, int *tile)
     return {start[0], start[r.experts]};
 }
 
+// A row's number, unsigned: all teams of a warp go round as often as the busiest, and one of the few that are left over begins behind the last row
+// and goes on by as much again and some steps, which is below 2^32 (2 kMostRows and 5 x 28416), where a signed number came back as one of a
+// row in front of the last (1.08 G rows of 288 columns).  A step that is 0 for those teams takes a register too many: 8192 x 28672 108 us for 100.
+using RowNumber = uint32_t;
+
 // What a team of lanes works on: 128 columns of some rows.  Of grouped rows it takes `most` in a row, so that the expert hardly ever
 // changes from one to the next (32768 x 2048 bf16 rows of 256 experts: 49 us with rows a grid apart, 38 so); of others rows a grid apart, which
 // memory takes better (8192 x 28672 fp32: 156 us, in a row 176).
 struct Walk {
-    int row, end, step, most, col;
-    int segment, segmentEnd;            // of a batch: its matrix; of grouped rows: the expert
+    RowNumber row, end;
+    int step, most, col;
+    int segment;
+    RowNumber segmentRow, segmentEnd;   // of a batch: its matrix; of grouped rows: the expert
     int64_t tileBase;                   // bytes to the segment's tiles of this column
-    int segmentRow;
     __device__ Walk(int lanes, const Range &range, const Rows &r, const int *start, const int *tile)
     {
         const int mine = (blockIdx.x * kThreads + threadIdx.x) / lanes, lane = mine / r.tileCols;         // lane: of those that take rows
@@ -61,7 +67,7 @@ struct Walk {
         most = r.offsets ? (rows + r.across - 1) / r.across : r.most;
         step = r.offsets ? 1 : r.across;
         const int64_t first = lane >= r.across ? rows : r.offsets ? (int64_t)lane * most : lane;         // the few teams that are left over have nothing to do
-        row = (int)(range.first + min(first, (int64_t)rows)); end = r.offsets ? (int)min((int64_t)row + most, range.last) : (int)range.last;
+        row = (RowNumber)(range.first + min(first, (int64_t)rows)); end = r.offsets ? (RowNumber)min((int64_t)row + most, range.last) : (RowNumber)range.last;
         segment = 0; segmentRow = 0; segmentEnd = end;
         tileBase = (int64_t)col * kTileBytes;
         if (row < end && (r.offsets || r.batch > 1)) {
@@ -73,7 +79,7 @@ struct Walk {
     {
         int64_t tileRow;
         if (r.offsets) { segmentRow = start[segment]; segmentEnd = start[segment + 1]; tileRow = tile[segment]; }
-        else { segmentRow = segment * (int)r.rows; segmentEnd = segmentRow + (int)r.rows; tileRow = segment * ((r.rows + kTileRows - 1) / kTileRows); }
+        else { segmentRow = segment * (RowNumber)r.rows; segmentEnd = segmentRow + (RowNumber)r.rows; tileRow = segment * ((r.rows + kTileRows - 1) / kTileRows); }
         tileBase = (tileRow * r.tileCols + col) * kTileBytes;
     }
     __device__ void Next(const Rows &r, const int *start, const int *tile)
@@ -342,21 +348,26 @@ HcclResult CheckRows(const char *what, int64_t batch, int64_t rows, int64_t cols
     return HCCL_SUCCESS;
 }
 
+// small operands: a chunk to every team of lanes, so that all loads are under way at once; large ones: as many blocks as fit
+// at once, since each builds the table of groups first (5003 x 2048 by 32 experts, eight blocks a SM: 12.5 us, five 10.0)
+int64_t SetGrid(Rows *r, int lanes, int blocks, int sms)
+{
+    const int teams = kThreads / lanes;
+    const int64_t rows = r->batch * r->rows, chunks = rows * r->tileCols;
+    const int64_t least = ((int64_t)r->tileCols + teams - 1) / teams;          // a row at a time needs so many
+    const int64_t grid = std::max(least, std::min<int64_t>((chunks + teams - 1) / teams, (int64_t)sms * blocks));
+    r->across = (int)(grid * teams / r->tileCols);
+    r->most = (int)((rows + r->across - 1) / r->across);
+    return grid;
+}
+
 // Programmatic launch: set-up overlaps the end of the kernel in front, which the kernel waits for before it touches memory.
 template <typename... Params, typename... Args> HcclResult Launch(const char *what, void (*kernel)(Rows, Params...), int lanes, int blocks, Rows r, void *stream, Args... args)
 {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchConfig_t cfg = {};
-    // small operands: a chunk to every team of lanes, so that all loads are under way at once; large ones: as many blocks as fit
-    // at once, since each builds the table of groups first (5003 x 2048 by 32 experts, eight blocks a SM: 12.5 us, five 10.0)
-    const int teams = kThreads / lanes;
-    const int64_t rows = r.batch * r.rows, chunks = rows * r.tileCols;
-    const int64_t least = ((int64_t)r.tileCols + teams - 1) / teams;           // a row at a time needs so many
-    const int64_t grid = std::max(least, std::min<int64_t>((chunks + teams - 1) / teams, (int64_t)sms * blocks));
-    r.across = (int)(grid * teams / r.tileCols);
-    r.most = (int)((rows + r.across - 1) / r.across);
-    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    cfg.gridDim = dim3((unsigned)SetGrid(&r, lanes, blocks, sms), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = r.experts > 0 ? 8 * (r.experts + 1) : 0;         // no more, so that a product behind finds room beside the last blocks
     cfg.stream = (cudaStream_t)stream;
@@ -436,4 +447,26 @@ extern "C" int HcommFp4Dequantize(const void *values, const void *scales, int64_
             RPT_ERR("EI0003", "HcommFp4Dequantize: data type %d is not FP32, FP16 or BFP16", dataType);
             return HCCL_E_PARA;
     }
+}
+
+// Whether a team of the quantiser's lanes takes its rows and no others, on a device of so many SMs and of rows without groups: followed in 64 bits
+// beside the kernel's own numbers for as long as it goes round.  Returns how many teams there are, of which the last ones may be left over; -1: no
+// such call, -2: it takes a row that is not its own.
+extern "C" int64_t HcommToolFp4Walk(int64_t rows, int64_t cols, int dataType, int sms, int64_t team)
+{
+    if (rows < 1 || cols < kBlock || CheckRows("HcommToolFp4Walk", 1, rows, cols, nullptr, 0) != HCCL_SUCCESS) return -1;
+    const bool fp8 = dataType == HCCL_DATA_TYPE_FP8E4M3;
+    const int lanes = fp8 ? kLanes<__nv_fp8_e4m3> : kLanes<float>, blocks = fp8 ? kBlocks<__nv_fp8_e4m3> : kBlocks<float>, together = 4;
+    Rows r{rows, cols, 1, (int)((cols + kTileCols - 1) / kTileCols), 0, 0, nullptr, 0};
+    const int64_t teams = SetGrid(&r, lanes, blocks, sms) * (kThreads / lanes), lane = team / r.tileCols;
+    int64_t at = lane < r.across ? std::min(lane, rows) : rows;
+    RowNumber row = (RowNumber)at;
+    const RowNumber end = (RowNumber)rows;
+    for (int left = r.most; left > 0; left -= together)
+        for (int u = 0; u < together; ++u) {
+            if (row < end && ((int64_t)row != at || at < 0)) return -2;
+            row = (RowNumber)((uint32_t)row + r.across);
+            at += r.across;
+        }
+    return teams;
 }

@@ -121,3 +121,20 @@ def test_products_refuse_a_depth_that_32_bits_cannot_round_up(k, gated):
     p = ctypes.c_void_p
     fn = _lib.load().HcommFp4GemmSwiglu if gated else _lib.load().HcommFp4Gemm
     assert fn(*[p(64)] * (6 if gated else 4), p(64), 1, 1, k, i64(1), p(0), 0, p(0)) == PARA
+
+
+@pytest.mark.parametrize("rows,cols", [((1 << 30) + (1 << 26), 288), ((1 << 31) - (1 << 20) - 1, 32), ((1 << 31) - (1 << 20) - 1, 288), ((1 << 31) - (1 << 20) - 1, 640), (1 << 30, 384), (5, 288),
+                                       (1, 32 * 200001), (100000, 8192)])
+@pytest.mark.parametrize("kind", [_lib.BF16, _lib.FP8E4M3])
+def test_no_team_of_the_quantiser_takes_a_row_that_is_not_its_own(rows, cols, kind):
+    """A team goes round as often as the busiest; the numbers of the rows behind the last one must not come back as those of others."""
+    cols = -(-cols // 128) * 128 if kind == _lib.FP8E4M3 else cols
+    walk = _lib.load().HcommToolFp4Walk
+    walk.restype = ctypes.c_int64
+
+    def follow(team):
+        return walk(i64(rows), i64(cols), kind, 148, i64(team))
+    teams = follow(0)
+    assert teams >= -(-cols // 128)
+    for team in (teams - 1, teams - 2, teams // 2, 1):
+        assert follow(team) == teams, team

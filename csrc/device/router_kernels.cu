@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(Threads<V>()) RouteBackwardKernel(const __grid
                 const float share = ChosenShare(value, chosen, p.sigmoid);
                 to = share * (dg - WarpSum(share * dg));
             } else if (p.sigmoid) to = chosen ? dg * expf(LogSigmoid(value)) : 0.f;
+            __syncwarp();                       // the token in front has cleared its places, by other lanes
             if (chosen) mine[expert] = to;
             __syncwarp();
             float own[V];

@@ -388,3 +388,25 @@ def test_a_coefficient_that_is_0_in_32_bits_makes_a_loss_of_0():
             loss = route(x, 2, balance=1e-50).loss
         assert loss is not None and loss.item() == 0
         assert torch.equal(torch.autograd.grad(loss, x)[0], torch.zeros_like(x))
+
+
+@pytest.mark.parametrize("e,k", [(64, 6), (256, 8), (1024, 16)])
+def test_gradients_of_tokens_that_share_experts_in_turn(e, k):
+    """A warp's tokens, one after the other, choose the same experts by other lanes: what one leaves in the row that they share is not the next one's."""
+    from hcomm_b200.ops.router import route
+    g = gen(e)
+    t = 148 * 2 * 32 * 3 + 5
+    order = torch.stack([torch.randperm(k, device="cuda", generator=g) for _ in range(16)])[torch.arange(t, device="cuda") // 32 % 16]
+    x = torch.randn(t, e, device="cuda", generator=g) * 0.1
+    x[:, ::e // k] = 0
+    x.scatter_(1, torch.arange(k, device="cuda") * (e // k) + torch.zeros_like(order), 3.0 + order * 0.25)
+    x.requires_grad_()
+    dgates = torch.randn(t, k, device="cuda", generator=g)
+    r = route(x, k, scale=SCALE)
+    share = torch.softmax(x.detach().double().gather(1, r.topk_idx.long()), 1)
+    none = torch.zeros((), device="cuda", dtype=torch.float64)
+    want, size = gradient(x.detach(), r.topk_idx.long(), share, torch.zeros(e, device="cuda"), t, torch.zeros_like(x, dtype=torch.float64), "softmax", True, dgates, none, k)
+    tol = (3 * relative(x.detach(), e) + 2.0 ** -21 + 2.0 ** -24) * size + 1e-37
+    for _ in range(3):
+        (dx,) = torch.autograd.grad(r.gates, x, dgates, retain_graph=True)
+        assert bool(((dx.double() - want).abs() <= tol).all())

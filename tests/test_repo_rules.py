@@ -86,3 +86,15 @@ def test_kernels_that_meet_other_ranks_let_nothing_start_early():
     lines = [ln for ln in text.splitlines() if "launch_dependents" in ln]
     assert lines and all("if (p.overlaps)" in ln for ln in lines)
     assert "hp.overlaps = m->comm->nRanks == 1;" in text
+
+
+def test_lanes_of_the_routing_gradient_meet_between_accesses_to_their_shared_row():
+    """Votes and shuffles do not order memory: between any two accesses of a token's row in shared memory, those of two tokens in a row
+    included, stands a barrier of the warp."""
+    text = (ROOT / "csrc" / "device" / "router_kernels.cu").read_text()
+    body = text[text.index("RouteBackwardKernel(const"):]
+    body = body[body.index("for (; t < p.tokens"):body.index("StoreRow<T, V>(d")]
+    steps = [("meet" if m.group(0).startswith("__") else "access") for m in re.finditer(r"__syncwarp\(\)|mine\[", body)]
+    assert steps.count("access") == 3
+    for here, after in zip(steps, steps[1:] + steps[:1]):
+        assert "meet" in (here, after), steps

@@ -28,6 +28,7 @@
 
 #include "../../include/hcomm_moe.h"
 #include "../core/log.h"
+#include "../core/per_device.h"
 #include "gemm_sm100_2sm.cuh"
 #include "sm100_ptx.cuh"
 
@@ -634,10 +635,6 @@ constexpr int kMostBlocks = 256;        // of scratch, whatever the device
 template <typename Kernel, typename... Args>
 HcclResult Launch(const char *what, Kernel *kernel, int grid, int cluster, int threads, int smem, void *stream, const Args &...args)
 {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-        HCCL_ERROR("%s: %d bytes of shared memory: %s", what, smem, cudaGetErrorString(cudaGetLastError()));
-        return HCCL_E_RUNTIME;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(threads, 1, 1);
@@ -657,12 +654,34 @@ HcclResult Launch(const char *what, Kernel *kernel, int grid, int cluster, int t
     }
     return HCCL_SUCCESS;
 }
+constexpr int SharedBytes(int v, int experts, bool backward, bool stats)
+{
+    const int warps = v >= 16 ? 16 : 32;
+    return backward ? warps * 32 * v * 4 : 4 * (experts + 1 + (stats ? warps * experts : 0));
+}
+// A kernel's limit of shared memory is the process's: it is raised once a GPU to the most that any call takes, never set to a call's own, or
+// another thread's launch finds it lower than what it asks for.
+template <typename T, int V, bool BACKWARD> HcclResult LaunchRows(const char *what, const Params &p, int grid, void *stream)
+{
+    constexpr auto kernel = BACKWARD ? RouteBackwardKernel<T, V> : RouteKernel<T, V>;
+    constexpr int most = SharedBytes(V, 32 * V, BACKWARD, true);
+    if constexpr (most > 48 * 1024) {
+        static hc::PerDevice<bool> allowed;
+        int dev = -1;
+        const bool good = cudaGetDevice(&dev) == cudaSuccess && allowed.Get(dev, [](bool *v) {
+            return *v = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) == cudaSuccess;
+        });
+        if (!good) {
+            HCCL_ERROR("%s: %d bytes of shared memory: %s", what, most, cudaGetErrorString(cudaGetLastError()));
+            return HCCL_E_RUNTIME;
+        }
+    }
+    return Launch(what, kernel, grid, 1, Threads<V>(), SharedBytes(V, p.experts, BACKWARD, p.partSums != nullptr), stream, p);
+}
 template <typename T, bool BACKWARD> HcclResult LaunchRows(const char *what, const Params &p, int grid, void *stream)
 {
-    const int v = ValuesOf(p.experts), warps = WarpsOf(v);
-    const int smem = BACKWARD ? warps * 32 * v * 4 : 4 * (p.experts + 1 + (p.partSums ? warps * p.experts : 0));
-    switch (v) {
-#define HCOMM_CASE(V) case V: return Launch(what, BACKWARD ? RouteBackwardKernel<T, V> : RouteKernel<T, V>, grid, 1, warps * 32, smem, stream, p);
+    switch (ValuesOf(p.experts)) {
+#define HCOMM_CASE(V) case V: return LaunchRows<T, V, BACKWARD>(what, p, grid, stream);
         HCOMM_CASE(1) HCOMM_CASE(2) HCOMM_CASE(4) HCOMM_CASE(8) HCOMM_CASE(16) HCOMM_CASE(32)
 #undef HCOMM_CASE
     }

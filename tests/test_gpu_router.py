@@ -410,3 +410,31 @@ def test_gradients_of_tokens_that_share_experts_in_turn(e, k):
     for _ in range(3):
         (dx,) = torch.autograd.grad(r.gates, x, dgates, retain_graph=True)
         assert bool(((dx.double() - want).abs() <= tol).all())
+
+
+def test_threads_whose_calls_need_different_shared_memory():
+    """Both sizes run the same kernel with more than 48 KB of shared memory; neither may lower what the other one is allowed."""
+    import threading
+    from hcomm_b200.ops.router import route
+    g = gen(33)
+    xs = [torch.randn(64, e, device="cuda", generator=g) for e in (800, 1024)]
+    want = [route(x, 8, balance=BALANCE) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        torch.cuda.set_device(0)
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3000):
+                    r = route(xs[i], 8, balance=BALANCE)
+                if not torch.equal(r.topk_idx, want[i].topk_idx) or not torch.equal(r.loss, want[i].loss):
+                    bad.append(i)
+        except RuntimeError as e:
+            bad.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1, 0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

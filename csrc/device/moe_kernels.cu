@@ -69,6 +69,7 @@ struct MoeParams {
     int segsPerItem;                      // sum: 256-column segments that a warp takes at a time
     int countsLaunch;                     // sum: this launch is the whole operator (single rank) and advances the launch state
     int allThroughSlots;                  // combine: rows of this rank's own tokens go through the landing area too
+    int nanGates;                         // sum: a gate of NaN counts although no row was sent for it
     int overlaps;                         // single rank: the kernel behind may take SMs early (see MOE_ARGS)
 };
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -516,8 +517,8 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtasPerSm) MoeCombineSumKerne
         if (i < items && lane < K && t < dispatched) {
             const size_t tk = (size_t)t * K + lane;
             nextRow = p.allThroughSlots ? 0u : p.localRow[tk];
-            nextValid = Valid(p, me)[tk];
             nextGate = p.gates[tk];
+            nextValid = Valid(p, me)[tk] | (p.nanGates && nextGate != nextGate);         // whatever lies in the slot: times NaN it is NaN
         }
     };
     int it = blockIdx.x * warpsPerCta + warp;
@@ -889,13 +890,7 @@ int HcommMoeDispatch(void *handle, const void *x, const int32_t *topkIdx, int nu
     return LaunchDispatch(m, hp, 9100, 9101, stream);
 }
 
-int HcommMoeCombine(void *handle, const void *y, const float *gates, void *out, int numTokens, void *stream)
-{
-    // how many rows y has is not known here: as many as can be received
-    return HcommMoeCombineRows(handle, y, handle ? (uint64_t)((MoeCtx *)handle)->lay.maxRecvRows : 0, gates, out, numTokens, stream);
-}
-
-int HcommMoeCombineRows(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, void *stream)
+static int Combine(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, bool nanGates, void *stream)
 {
     MoeCtx *m = (MoeCtx *)handle;
     if (!m || !y || !gates || !out) return HCCL_E_PTR;
@@ -908,6 +903,7 @@ int HcommMoeCombineRows(void *handle, const void *y, uint64_t yRows, const float
     MoeParams hp;
     FillCommon(m, hp);
     hp.y = (const __nv_bfloat16 *)y; hp.gates = gates; hp.out = (__nv_bfloat16 *)out; hp.numTokens = numTokens;
+    hp.nanGates = nanGates;
     ++c->opSeq;
     const uintptr_t yBegin = (uintptr_t)y, yEnd = yBegin + yRows * m->lay.hidden * 2;
     const uintptr_t outBegin = (uintptr_t)out, outEnd = outBegin + (uint64_t)numTokens * m->lay.hidden * 2;
@@ -926,6 +922,22 @@ int HcommMoeCombineRows(void *handle, const void *y, uint64_t yRows, const float
     const int64_t items = (int64_t)numTokens * ((segs + hp.segsPerItem - 1) / hp.segsPerItem);
     const int forced = ForcedMoeCtas(), most = forced > 0 ? forced : kSumCtasPerSm * sms;
     return LaunchMoe(m, SumKernel(m->lay.topk, c->emuSameDevice && c->nRanks > 1), hp, 9104, stream, (int)std::max<int64_t>(1, std::min<int64_t>(most, (items + warps - 1) / warps)), emuCtas, kSumThreads);
+}
+
+int HcommMoeCombine(void *handle, const void *y, const float *gates, void *out, int numTokens, void *stream)
+{
+    // how many rows y has is not known here: as many as can be received
+    return Combine(handle, y, handle ? (uint64_t)((MoeCtx *)handle)->lay.maxRecvRows : 0, gates, out, numTokens, false, stream);
+}
+
+int HcommMoeCombineRows(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, void *stream)
+{
+    return Combine(handle, y, yRows, gates, out, numTokens, false, stream);
+}
+
+int HcommMoeCombineRouted(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, void *stream)
+{
+    return Combine(handle, y, yRows, gates, out, numTokens, true, stream);
 }
 
 // ------------------------------------------------------------------ dispatch without any allocation

@@ -23,7 +23,7 @@ from ..comm import Communicator
 
 
 _short_dispatch = Short("moe_dispatch", "HcommMoeDispatch")
-_short_combine = Short("moe_combine", "HcommMoeCombineRows")
+_short_combine, _short_combine_routed = Short("moe_combine", "HcommMoeCombineRows"), Short("moe_combine", "HcommMoeCombineRouted")
 
 
 class MoeLayout(ctypes.Structure):
@@ -92,8 +92,10 @@ class MoeExchange:
                                               ctypes.c_void_p(stream)), "HcommMoeDispatch")
         return Received(self._rows, self._scales, self._origin, self._offsets)
 
-    def combine(self, y: torch.Tensor, gates: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        r = _short_combine(self._h.value, y, gates, out, self.hidden)
+    def combine(self, y: torch.Tensor, gates: torch.Tensor, out: torch.Tensor | None = None, *, nan_gates: bool = False) -> torch.Tensor:
+        """Gate-weighted sum of each token's rows.  A choice that dispatch did not send adds nothing, whatever its gate; with ``nan_gates`` one whose gate
+        is NaN makes its token NaN: ``ops.router.route`` gives a token whose logits are no numbers choices of -1 and gates of NaN."""
+        r = (_short_combine_routed if nan_gates else _short_combine)(self._h.value, y, gates, out, self.hidden)
         if r is not None:
             return r
         assert y.dtype == torch.bfloat16 and y.is_contiguous() and y.shape[1] == self.hidden
@@ -102,8 +104,9 @@ class MoeExchange:
         if out is None:
             out = torch.empty((t, self.hidden), dtype=torch.bfloat16, device=y.device)
         stream = raw_stream(y)
-        _lib.check(self._lib.HcommMoeCombineRows(self._h, ctypes.c_void_p(y.data_ptr()), ctypes.c_uint64(y.shape[0]), ctypes.c_void_p(gates.data_ptr()),
-                                                 ctypes.c_void_p(out.data_ptr()), t, ctypes.c_void_p(stream)), "HcommMoeCombineRows")
+        name = "HcommMoeCombineRouted" if nan_gates else "HcommMoeCombineRows"
+        _lib.check(getattr(self._lib, name)(self._h, ctypes.c_void_p(y.data_ptr()), ctypes.c_uint64(y.shape[0]), ctypes.c_void_p(gates.data_ptr()),
+                                            ctypes.c_void_p(out.data_ptr()), t, ctypes.c_void_p(stream)), name)
         return out
 
     def overflow(self) -> int:

@@ -3,7 +3,7 @@
     r = route(x @ w_router.T, topk=8, balance=0.01)         # logits [T, experts]
     recv = moe.dispatch(x, r.topk_idx)
     ... the experts ...
-    out = moe.combine(y, r.gates)
+    out = moe.combine(y, r.gates, nan_gates=True)
     loss = task_loss + r.loss
 
 ``gates`` and ``loss`` have gradients with regard to the logits; choices and counts are constants.  With f_e the share of the
@@ -143,7 +143,8 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", renormal
     comm         counts and loss over the tokens of all ranks of a communicator (a collective call); each rank's gradient is that of
                  the one loss with regard to its own logits
 
-    A logit of -inf takes the expert out for the token.  A row that holds a NaN (under softmax: or +inf) chooses -1 with gates of NaN."""
+    A logit of -inf takes the expert out for the token.  A row that holds a NaN (under softmax: or +inf) chooses -1 with gates of NaN,
+    which ``MoeExchange.combine(..., nan_gates=True)`` carries on."""
     if comm is None and topk.__class__ is int and scoring in SCORINGS:
         r = _short_route(logits, topk, SCORINGS[scoring], 1 if renormalize else 0, float(scale), bias, valid, float(balance))
         if r is not None:

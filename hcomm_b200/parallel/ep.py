@@ -60,7 +60,7 @@ class ExpertParallelMlp:
         offsets = recv.expert_offsets
         h = gemm_fp4_swiglu(quantize_fp4(recv.rows, recv.scales, offsets=offsets), self.gate, self.up, self._h)
         y = gemm_fp4(quantize_fp4(h, offsets=offsets), self.down, self._y)
-        return self.moe.combine(y, r.gates, out)
+        return self.moe.combine(y, r.gates, out, nan_gates=True)
 
     __call__ = forward
 

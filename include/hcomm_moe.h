@@ -43,6 +43,9 @@ int HcommMoeDispatch(void *handle, const void *x, const int32_t *topkIdx, int nu
  * capacity, and takes a result that starts behind a shorter y for one inside it (same result, a pass more). */
 int HcommMoeCombine(void *handle, const void *y, const float *gates, void *out, int numTokens, void *stream);
 int HcommMoeCombineRows(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, void *stream);
+/* HcommMoeCombineRows with the gates of HcommMoeRoute, which gives a token whose logits are no numbers choices of -1 and gates of NaN: a token with a
+ * gate of NaN comes back as NaN, also where no row was sent for it (the other two leave such a gate out, whatever it holds). */
+int HcommMoeCombineRouted(void *handle, const void *y, uint64_t yRows, const float *gates, void *out, int numTokens, void *stream);
 /* Rows dropped because a rank received more than its capacity since the last call (clears the counter). */
 int HcommMoeTakeOverflow(void *handle);
 

@@ -140,3 +140,89 @@ def test_refusals():
         with pytest.raises(ValueError):
             ExpertParallelMlp(comm, **{**dict(experts=8, topk=2, hidden=512, intermediate=64, max_tokens=8), **bad})
     comm.destroy()
+
+
+def _with_tokens_that_are_no_numbers(g, tokens, hidden):
+    """x, which of its tokens are, and x without them."""
+    x = torch.randn(tokens, hidden, device="cuda", generator=g).to(torch.bfloat16)
+    bad = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    bad[[0, 3, tokens - 2]] = True
+    clean = x.clone()
+    x[0, 5], x[3], x[tokens - 2, :2] = float("nan"), float("nan"), torch.tensor([float("inf"), float("-inf")], device="cuda")
+    return x, bad, clean
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_a_token_that_is_no_number_comes_back_as_such(scoring):
+    g = gen(91)
+    comms, (layer,) = make(1, experts=16, topk=4, hidden=512, intermediate=96, max_tokens=70, scoring=scoring)
+    try:
+        x, bad, clean = _with_tokens_that_are_no_numbers(g, 70, 512)
+        # weights of both signs: an infinite logit of each sign, or inf - inf; softmax knows neither, sigmoid not the latter
+        layer.router.copy_(torch.randn(16, 512, device="cuda", generator=g).to(torch.bfloat16) * 0.02)
+        layer.router[:, :2] = torch.tensor([[1.0, 1.0], [1.0, -1.0]], device="cuda").repeat(8, 1).to(torch.bfloat16)
+        want = layer(clean).clone()
+        out = layer(x).clone()
+        assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], want[~bad]) and not torch.isnan(want).any()
+        # padding is not looked at, and the next batch does not know
+        padded = layer(x, valid=~bad).clone()
+        assert not padded[bad].any() and torch.equal(padded[~bad], want[~bad])
+        assert torch.equal(layer(clean), want)
+        graph, into = torch.cuda.CUDAGraph(), torch.empty_like(out)
+        with torch.cuda.graph(graph):
+            layer(x, into)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(into[~bad], want[~bad]) and torch.isnan(into[bad]).all()
+    finally:
+        end(comms, [layer])
+
+
+def test_a_token_that_is_no_number_on_one_of_two_ranks():
+    g = gen(92)
+    comms, layers = make(2, experts=16, topk=4, hidden=512, intermediate=96, max_tokens=40)
+    x, bad, clean = _with_tokens_that_are_no_numbers(g, 40, 512)
+
+    def run(batches):
+        def step(r):
+            torch.cuda.set_device(0)
+            out = layers[r](batches[r])
+            torch.cuda.synchronize()
+            return out.clone()
+        return run_ranks(2, step)
+    want, got = run([clean, clean]), run([x, clean])
+    assert torch.isnan(got[0][bad]).all() and torch.equal(got[0][~bad], want[0][~bad]) and torch.equal(got[1], want[1])
+    end(comms, layers)
+
+
+@pytest.mark.parametrize("through_slots", [False, True])
+def test_combine_carries_gates_that_are_no_numbers_where_it_is_asked_to(through_slots):
+    import contextlib
+    import hcomm_b200 as hb
+    from hcomm_b200.ops.moe import MoeExchange
+    g = gen(93)
+    comm = hb.Communicator(1, hb.get_root_info(), 0, buffer_mb=4)
+    moe = MoeExchange(comm, 8, 2, 512, 50)
+    try:
+        x = torch.randn(50, 512, device="cuda", generator=g).to(torch.bfloat16)
+        idx = torch.randint(0, 8, (50, 2), device="cuda", generator=g, dtype=torch.int32)
+        idx[::5] = -1
+        idx[1::5, 1] = -1
+        recv = moe.dispatch(x, idx)
+        y = torch.randn(recv.num_rows + 50, 512, device="cuda", generator=g).to(torch.bfloat16)
+        gates = torch.rand(50, 2, device="cuda", generator=g)
+        gates[idx < 0] = 0
+        want = moe.combine(y, gates).clone()
+        gates[::5] = float("nan")
+        gates[1::10, 1] = float("nan")
+        bad = torch.isnan(gates).any(1)
+        for mode in (contextlib.nullcontext(), torch.overrides.BaseTorchFunctionMode()):        # the native call, and the general one
+            with mode:
+                carried, left_out = y.clone(), y.clone()
+                carried = moe.combine(carried, gates, carried[-50:] if through_slots else None, nan_gates=True)
+                left_out = moe.combine(left_out, gates, left_out[-50:] if through_slots else None)
+            assert torch.isnan(carried[bad]).all() and torch.equal(carried[~bad], want[~bad])
+            assert torch.equal(left_out, want)          # as ever: a choice that was not sent adds nothing
+    finally:
+        moe.destroy()
+        comm.destroy()

@@ -263,6 +263,7 @@ PyObject *Route(PyObject *, PyObject *const *args, Py_ssize_t n)
     const int dev = Device();
     const Tensor *x = dev < 0 ? nullptr : Plain(args[3], dev);
     if (!x || x->dim() != 2 || (x->scalar_type() != at::kFloat && x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
+    if (x->_fw_grad(0).defined()) Py_RETURN_NONE;       // forward mode, which the general way refuses
     void *f, *b, *s;
     if (!Address(args[0], &f) || !Address(args[1], &b) || !Address(args[2], &s)) Py_RETURN_NONE;
     const long topk = PyLong_AsLong(args[4]);           // whole: 2^32 + 2 is not 2

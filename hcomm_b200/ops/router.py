@@ -6,7 +6,7 @@
     out = moe.combine(y, r.gates, nan_gates=True)
     loss = task_loss + r.loss
 
-``gates`` and ``loss`` have gradients with regard to the logits; choices and counts are constants.  With f_e the share of the
+``gates`` and ``loss`` have gradients with regard to the logits (in reverse mode, once); choices and counts are constants.  With f_e the share of the
 tokens' choices that went to expert e and P_e the tokens' mean probability of it, the loss is ``balance * experts * sum f_e P_e``, which is
 ``balance`` where both are even.
 """
@@ -17,6 +17,7 @@ import operator
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -174,5 +175,7 @@ def route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax", renormal
             raise ValueError(f"valid must be bool [{t}] on {logits.device}")
         valid = valid.contiguous()
     args = (logits, topk, SCORINGS[scoring], bool(renormalize), float(scale), bias, valid, float(balance), comm)
-    idx, gates, counts, loss = _Route.apply(*args) if logits.requires_grad and torch.is_grad_enabled() else _forward(*args)
+    # a tangent of forward mode goes to the function as well, which has none to offer and says so
+    followed = (logits.requires_grad and torch.is_grad_enabled()) or unpack_dual(logits).tangent is not None
+    idx, gates, counts, loss = _Route.apply(*args) if followed else _forward(*args)
     return Routing(idx, gates, counts[:e], loss)

@@ -438,3 +438,17 @@ def test_threads_whose_calls_need_different_shared_memory():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_a_tangent_is_refused_and_not_dropped(requires_grad):
+    import torch.autograd.forward_ad as fwad
+    from hcomm_b200.ops.router import route
+    x = torch.randn(6, 8, device="cuda", requires_grad=requires_grad)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for mode in (contextlib.nullcontext(), torch.overrides.BaseTorchFunctionMode(), torch.no_grad()):        # the native call, the general one, without reverse mode
+            with mode, pytest.raises(RuntimeError, match="jvp"):
+                route(dual, 2, balance=BALANCE)
+        assert route(x, 2).topk_idx.shape == (6, 2)         # no tangent, no refusal
+    assert torch.equal(route(dual, 2).topk_idx, route(x, 2).topk_idx)

@@ -432,3 +432,92 @@ def test_depths_beyond_32_bits_are_refused_by_every_way():
                 gemm_fp4(q, q)
             with pytest.raises(ValueError, match="at most"):
                 gemm_fp4_swiglu(q, q, q)
+
+
+def fp8_rows(g, rows, cols, scales):
+    """Codes of every kind but NaN, and scales [rows, cols // 128] of the given kind."""
+    codes = torch.randint(0, 256, (rows, cols), device="cuda", generator=g, dtype=torch.uint8)
+    codes[(codes & 127) == 127] = 3
+    return codes.view(torch.float8_e4m3fn), scales.expand(rows, cols // 128).float().contiguous()
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 3, 3, 140, 150]])
+@pytest.mark.parametrize("low,high", [(-149, -120), (-127, -100), (-80, -55), (-66, -62), (100, 118)])
+def test_exchanged_rows_of_every_magnitude(low, high, offsets):
+    """Products below the range of ordinary numbers, and on both sides of the border (block scales of 2^-63) where the multiplier is taken into the
+    block's power of two instead of into every value; scales that are no powers of two, and negative ones."""
+    from hcomm_b200.ops.fp4 import dequantize_fp4, quantize_fp4
+    g = gen(71 - low)
+    rows, cols = 150, 512
+    power = torch.randint(low, high + 1, (rows, cols // 128), device="cuda", generator=g)
+    mantissa = 1 + torch.rand(rows, cols // 128, device="cuda", generator=g, dtype=torch.float64)
+    sign = torch.where(torch.rand(rows, cols // 128, device="cuda", generator=g) < 0.3, -1.0, 1.0)
+    x, scales = fp8_rows(g, rows, cols, (sign * torch.ldexp(mantissa, power)).float())
+    # blocks of small codes beside the others, so that the largest product is far below 448 of its scale
+    small = torch.randint(0, 9, (rows, cols), device="cuda", generator=g, dtype=torch.uint8) + 128 * torch.randint(0, 2, (rows, cols), device="cuda", generator=g, dtype=torch.uint8)
+    pick = (torch.rand(rows, cols // 32, device="cuda", generator=g) < 0.4).repeat_interleave(32, 1)
+    x = torch.where(pick, small, x.view(torch.uint8)).view(torch.float8_e4m3fn)
+    want = nearest((x.double() * scales.double().repeat_interleave(128, 1)).float())        # a value is the product rounded to fp32, once
+    at = None if offsets is None else torch.tensor(offsets, device="cuda", dtype=torch.int32)
+    q = quantize_fp4(x, scales, offsets=at)
+    assert same(dequantize_fp4(q, torch.float32), want)
+    if at is None:
+        assert same(held(q), want)
+        border = q.block_scales()
+        assert (low, high) != (-80, -55) or ((border == 63).any() and (border == 64).any())
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 3, 3, 140, 150]])
+def test_exchanged_rows_that_are_no_numbers(offsets):
+    from hcomm_b200.ops.fp4 import dequantize_fp4, quantize_fp4
+    g = gen(72)
+    x, scales = fp8_rows(g, 150, 512, torch.ones(150, 4, device="cuda"))
+    for row, value in enumerate((0.0, -0.0, float("inf"), float("-inf"), float("nan"), torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max, 1e-45, 2.0 ** -126)):
+        scales[10 + row, 1], scales[60 + row, :] = value, value
+    x.view(torch.uint8)[100, 40], x.view(torch.uint8)[101, 511], x.view(torch.uint8)[102, :32] = 0x7f, 0xff, 0x7f
+    x.view(torch.uint8)[62, 128:256] = 0          # no numbers: zero times infinity
+    scales[103, 0], x.view(torch.uint8)[103, 5] = 0.0, 0x7f
+    want = nearest((x.double() * scales.double().repeat_interleave(128, 1)).float())
+    at = None if offsets is None else torch.tensor(offsets, device="cuda", dtype=torch.int32)
+    q = quantize_fp4(x, scales, offsets=at)
+    assert same(dequantize_fp4(q, torch.float32), want)
+    bad = torch.isnan(want.view(150, 16, 32)).any(2)
+    for row, blocks in ((12, 4), (13, 4), (14, 4), (62, 16), (63, 16), (64, 16), (100, 1), (101, 1), (102, 1), (103, 1), (10, 0), (11, 0), (60, 0), (67, 0)):
+        assert int(bad[row].sum()) == blocks, row
+
+
+@pytest.mark.parametrize("m,n,k,grouped", [(9, 40, 64, False), (1, 256, 8192, False), (300, 136, 96, False), (1000, 1000, 64, True)])
+def test_gates_far_below_zero(m, n, k, grouped):
+    """silu is 0 below -87.3, where its magnitude is under 2^-119: beside what a gated product is off by anyway, up times that.  Infinite gates give what
+    the formula gives."""
+    from hcomm_b200.ops.fp4 import Fp4Tensor, gemm_fp4_swiglu, quantize_fp4
+    g = gen(m + n)
+    x = torch.randn(m, k, device="cuda", generator=g)
+    gate, up = torch.randn(n, k, device="cuda", generator=g), torch.randn(n, k, device="cuda", generator=g)
+    spread_out = torch.tensor([-60.0, -80.0, -86.0, -88.0, -90.0, -200.0, -3e4, 90.0, 3e4], device="cuda")
+    x[:, :32] = 0
+    x[:, 0] = 4.0
+    gate[:, :32] = 0
+    gate[:, 0] = spread_out[torch.arange(n, device="cuda") % 9] / 4.0
+    gate[:, 32:] *= 2.0 ** -6
+    a, w, u = quantize_fp4(x), quantize_fp4(gate), quantize_fp4(up)
+    args = (a, w, u)
+    if grouped:
+        args = (quantize_fp4(x, offsets=torch.tensor([0, m], device="cuda", dtype=torch.int32)), *(Fp4Tensor(q.values[None], q.scales) for q in (w, u)))
+    out = gemm_fp4_swiglu(*args).double()
+    want, tol = swiglu_reference(held(a), held(w), held(u))
+    ups = (held(a) @ held(u).t()).abs() + k * 2.0 ** -23 * (held(a).abs() @ held(u).abs().t())
+    far = (held(a) @ held(w).t()) < -80
+    assert far.any() and bool(((out - want).abs() <= tol + far * 2.0 ** -119 * ups).all())
+    # beyond the range of 32 bits
+    huge = torch.zeros(2, k, device="cuda")
+    huge[:, 0] = torch.tensor([3e38, -3e38], device="cuda")
+    x[:] = 0
+    x[:, 0], x[:, 1] = 2.0 ** 10, 1.0
+    up[:] = 0
+    up[:, 1] = 3.0
+    # the one shares its power of two, 2^8, with the 2^10 and becomes 0: infinity times up's 0, and -inf 0
+    assert torch.isnan(gemm_fp4_swiglu(quantize_fp4(x), quantize_fp4(huge), quantize_fp4(up[:2]))).all()
+    x[:, 40], up[:, 40] = 1.0, 3.0          # a block of their own: up is 3
+    out = gemm_fp4_swiglu(quantize_fp4(x), quantize_fp4(huge), quantize_fp4(up[:2]))
+    assert (out[:, 0] == float("inf")).all() and torch.isnan(out[:, 1]).all()          # inf 1 3; -inf 0

@@ -452,3 +452,33 @@ def test_a_tangent_is_refused_and_not_dropped(requires_grad):
                 route(dual, 2, balance=BALANCE)
         assert route(x, 2).topk_idx.shape == (6, 2)         # no tangent, no refusal
     assert torch.equal(route(dual, 2).topk_idx, route(x, 2).topk_idx)
+
+
+def test_saved_tensors_pass_hooks_and_checkpoints():
+    """What the gradient needs is saved as any operator's is: hooks may keep it elsewhere, a checkpoint may make it again."""
+    from torch.utils.checkpoint import checkpoint
+    from hcomm_b200.ops.router import route
+    g = gen(44)
+    wide, valid = make(g, 300, 96, torch.bfloat16, True)
+    x = wide[:, :64].detach().requires_grad_()
+    dgates = torch.randn(300, 6, device="cuda", generator=g)
+
+    def loss(v):
+        r = route(v * 1.5, 6, valid=valid, balance=BALANCE)
+        return (r.gates * dgates).sum() + 7 * r.loss
+    (want,) = torch.autograd.grad(loss(x), x)
+    assert want.abs().sum() > 0
+    for mode in (contextlib.nullcontext(), torch.overrides.BaseTorchFunctionMode()):
+        with mode:
+            packed = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t.shape) or t.cpu(), lambda t: t.cuda()):
+                kept = loss(x)
+            assert packed.count((300, 64)) >= 1 and packed.count((300, 6)) >= 1
+            assert torch.equal(torch.autograd.grad(kept, x)[0], want)
+            with torch.autograd.graph.save_on_cpu():
+                kept = loss(x)
+            assert torch.equal(torch.autograd.grad(kept, x)[0], want)
+            for reentrant in (False, True):
+                y = x.detach().requires_grad_()
+                checkpoint(loss, y, use_reentrant=reentrant).backward()
+                assert torch.equal(y.grad, want)

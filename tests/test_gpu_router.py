@@ -482,3 +482,43 @@ def test_saved_tensors_pass_hooks_and_checkpoints():
                 y = x.detach().requires_grad_()
                 checkpoint(loss, y, use_reentrant=reentrant).backward()
                 assert torch.equal(y.grad, want)
+
+
+@pytest.mark.parametrize("scoring,renormalize", [("softmax", True), ("softmax", False), ("sigmoid", True)])
+@pytest.mark.parametrize("sizes", [(40, 3000), (3000, 0), (1, 33)])
+def test_one_loss_of_two_ranks(sizes, scoring, renormalize):
+    """Counts and loss are those of both ranks' tokens, and each rank's gradient is that of the one loss."""
+    import hcomm_b200 as hb
+    from hcomm_b200.ops.router import route
+    from helpers import run_ranks
+    g = gen(sum(sizes))
+    e, k = 64, 6
+    x, valid = make(g, sum(sizes), e, torch.float32, True)
+    dgates, dloss = torch.randn(sum(sizes), k, device="cuda", generator=g), torch.tensor(1.3 * sum(sizes), device="cuda")
+    idx, share, counts, tokens, p = reference(x, k, scoring, renormalize, None, valid)
+    rel = relative(x, e)
+    want = loss_of(counts, tokens, p, k)
+    want_dx, size = gradient(x, idx, share, counts, tokens, p, scoring, renormalize, dgates, dloss.double(), k)
+    tol = (3 * rel + 2.0 ** -21 + 2.0 ** -24) * size + 1e-37
+    spans = (slice(0, sizes[0]), slice(sizes[0], sum(sizes)))
+    info = hb.get_root_info()
+    comms = run_ranks(2, lambda r: (torch.cuda.set_device(0), hb.Communicator(2, info, r, buffer_mb=4))[1])
+    torch.cuda.synchronize()
+
+    def step(r):
+        torch.cuda.set_device(0)
+        mine = x[spans[r]].clone().requires_grad_()
+        out = route(mine, k, scoring=scoring, renormalize=renormalize, scale=SCALE, valid=valid[spans[r]], balance=BALANCE, comm=comms[r])
+        (dx,) = torch.autograd.grad((out.gates, out.loss), mine, (dgates[spans[r]], dloss))
+        without = route(mine.detach(), k, scoring=scoring, renormalize=renormalize, scale=SCALE, valid=valid[spans[r]], comm=comms[r])
+        torch.cuda.synchronize()
+        assert without.loss is None and torch.equal(without.counts, out.counts) and torch.equal(without.topk_idx, out.topk_idx)
+        return out, dx
+    for _ in range(2):
+        got = run_ranks(2, step)
+        for r, (out, dx) in enumerate(got):
+            assert torch.equal(out.topk_idx.long(), idx[spans[r]]) and torch.equal(out.counts.long(), counts)
+            assert abs(out.loss.double() - want) <= want * (rel + 2.0 ** -24 * (sum(sizes) / 32 + 401 + e))
+            assert bool(((dx.double() - want_dx[spans[r]]).abs() <= tol[spans[r]]).all())
+        assert torch.equal(got[0][0].loss, got[1][0].loss)
+    run_ranks(2, lambda r: comms[r].destroy())

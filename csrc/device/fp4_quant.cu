@@ -104,7 +104,7 @@ template <typename T> __device__ __forceinline__ void Load(Sixteen<T> *v, const 
 {
     if (aligned) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T); ++i) v->q[i] = __ldg((const uint4 *)p + i);
+        for (int i = 0; i < (int)sizeof(T); ++i) v->q[i] = ((const uint4 *)p)[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) ((T *)v)[i] = p[i];
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks<T>) QuantizeKernel(Rows r, S
                     const int64_t from = r.batch > 1 ? w.segment * s.batchPitch + (w.row - w.segmentRow) * s.rowPitch : w.row * s.rowPitch;
 #pragma unroll
                     for (int h = 0; h < P; ++h) Load(&in[u][h], (const T *)s.x + from + at + 16 * h, s.aligned);
-                    if constexpr (sizeof(T) == 1) mul[u] = __ldg(s.xScales + w.row * s.scalePitch + w.col);
+                    if constexpr (sizeof(T) == 1) mul[u] = s.xScales[w.row * s.scalePitch + w.col];
                     to[u] = values + (w.row * r.cols + at) / 2;
                 }
             }
@@ -314,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) DequantizeKernel(Rows r
         for (int u = 0; u < U; ++u) {
             at[u] = w.row < w.end ? w.row * r.cols + col : -1;
             if (at[u] >= 0) {
-                word[u] = __ldg((const uint2 *)(values + at[u] / 2));
-                byte[u] = __ldg(scales + w.Scales(r) + (lane >> 1));
+                word[u] = *(const uint2 *)(values + at[u] / 2);
+                byte[u] = scales[w.Scales(r) + (lane >> 1)];
             }
             w.Next(r, start, tile);
         }

@@ -83,7 +83,7 @@ template <typename T, int V> __device__ __forceinline__ void AskRow(Raw<T, V> &r
     if (vectors) {
         if (first < experts) {
 #pragma unroll
-            for (int i = 0; i < kBytes / kWord; ++i) ((W *)raw.v)[i] = __ldg((const W *)(row + first) + i);
+            for (int i = 0; i < kBytes / kWord; ++i) ((W *)raw.v)[i] = ((const W *)(row + first))[i];
         }
     } else {
 #pragma unroll

@@ -98,3 +98,15 @@ def test_lanes_of_the_routing_gradient_meet_between_accesses_to_their_shared_row
     assert steps.count("access") == 3
     for here, after in zip(steps, steps[1:] + steps[:1]):
         assert "meet" in (here, after), steps
+
+
+def test_kernels_resident_early_read_through_ordinary_loads():
+    """A kernel that may be resident before the kernel in front has ended lives while that one still writes what it reads: loads of the
+    read-only path, which is for memory that no one writes for as long as the kernel lives, have no place in it."""
+    seen = 0
+    for p in SOURCES:
+        text = p.read_text(errors="ignore")
+        if p.suffix in (".cu", ".cuh") and ("GridDependencyWait();" in text or "griddepcontrol.wait" in text):
+            seen += 1
+            assert "__ldg" + "(" not in text and "ld.global." + "nc" not in text, p
+    assert seen >= 6

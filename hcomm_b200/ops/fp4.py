@@ -53,22 +53,22 @@ class Fp4Tensor:
             raise TypeError("values and scales must be uint8, values of two or three dimensions")
         if values.shape[:-1] != scales.shape[:-1] or values.shape[-1] != 16 * scales.shape[-1] or values.device != scales.device:
             raise ValueError(f"values {tuple(values.shape)} and scales {tuple(scales.shape)} do not belong together")
-        rows, blocks = scales.shape[-2:]
-        s = scales.reshape(-1, rows, blocks)
+        *batch, rows, blocks = scales.shape
+        s = scales.reshape(batch[0] if batch else 1, rows, blocks)          # in figures: -1 says nothing about an empty one
         if blocks % 4 or rows % 128:
             s = torch.nn.functional.pad(s, (0, -blocks % 4, 0, -rows % 128))
         s = s.view(s.shape[0], s.shape[1] // 128, 4, 32, s.shape[2] // 4, 4).permute(0, 1, 4, 3, 2, 5)
         values = values.contiguous()
-        return cls(values if values.data_ptr() % 16 == 0 else values.clone(), s.reshape(-1, 512).contiguous())
+        return cls(values if values.data_ptr() % 16 == 0 else values.clone(), s.reshape(s.shape[:3].numel(), 512).contiguous())
 
     def block_scales(self) -> torch.Tensor:
         """The scales as ``from_parts`` takes them, [..., rows, cols // 32]; not of grouped rows."""
         if self.offsets is not None:
             raise ValueError("rows grouped by expert have their scales in the experts' tiles")
         *batch, rows, cols = self.shape
-        tiles = -(-rows // 128)
-        s = self.scales.view(-1, tiles, -(-cols // 128), 32, 4, 4).permute(0, 1, 4, 3, 2, 5)
-        return s.reshape(s.shape[0], tiles * 128, -1)[:, :rows, :cols // 32].reshape(*batch, rows, cols // 32)
+        matrices, down, across = batch[0] if batch else 1, -(-rows // 128), -(-cols // 128)
+        s = self.scales.view(matrices, down, across, 32, 4, 4).permute(0, 1, 4, 3, 2, 5)
+        return s.reshape(matrices, down * 128, across * 4)[:, :rows, :cols // 32].reshape(*batch, rows, cols // 32)
 
 
 def _on_device(what: str, *tensors) -> torch.device:

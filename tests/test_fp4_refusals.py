@@ -138,3 +138,13 @@ def test_no_team_of_the_quantiser_takes_a_row_that_is_not_its_own(rows, cols, ki
     assert teams >= -(-cols // 128)
     for team in (teams - 1, teams - 2, teams // 2, 1):
         assert follow(team) == teams, team
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (4, 0), (0, 4, 64), (3, 0, 64), (3, 4, 0)])
+def test_parts_of_nothing(shape):
+    """What quantize_fp4 makes of an empty matrix: an expert that a rank does not have, or a layer without rows."""
+    scales = torch.zeros((*shape[:-1], shape[-1] // 32), dtype=torch.uint8)
+    q = Fp4Tensor.from_parts(torch.zeros((*shape[:-1], shape[-1] // 2), dtype=torch.uint8), scales)
+    *batch, rows, cols = shape
+    assert q.shape == shape and q.scales.shape == (_scale_tiles(batch[0] if batch else 1, rows, cols, 0), 512)
+    assert torch.equal(q.block_scales(), scales)

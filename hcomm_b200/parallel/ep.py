@@ -52,6 +52,7 @@ class ExpertParallelMlp:
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, valid: torch.Tensor | None = None) -> torch.Tensor:
         """x [tokens, hidden] bf16; tokens that ``valid`` (bool [tokens]) takes out go to no expert and come back as 0.  A rank without
         tokens takes part all the same, as the pass is collective: with one that is taken out."""
+        self._check(x, out)
         if x.shape[0] == 0:
             self.forward(x.new_zeros((1, x.shape[1])), valid=torch.zeros(1, dtype=torch.bool, device=x.device))
             return torch.empty_like(x) if out is None else out
@@ -63,6 +64,16 @@ class ExpertParallelMlp:
         return self.moe.combine(y, r.gates, out, nan_gates=True)
 
     __call__ = forward
+
+    def _check(self, x, out):
+        """Before anything is queued: the exchange behind is a collective call, and writes where it is told to."""
+        hidden = self.router.shape[1]
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != hidden or not x.is_contiguous() or x.device != self.router.device:
+            raise ValueError(f"x must be contiguous bfloat16 [tokens, {hidden}] on {self.router.device}")
+        if x.shape[0] > self.moe.max_tokens:
+            raise ValueError(f"{x.shape[0]} tokens: the layer was made for {self.moe.max_tokens}")
+        if out is not None and (out.dtype != torch.bfloat16 or out.shape != x.shape or not out.is_contiguous() or out.device != x.device):
+            raise ValueError(f"out must be contiguous bfloat16 {list(x.shape)} on {x.device}")
 
     def destroy(self):
         self.moe.destroy()

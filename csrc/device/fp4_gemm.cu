@@ -101,7 +101,8 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 // Whether a product goes by pairs of CTAs (tiles of 256 rows x 256 columns, or 128 of a gated product) or by single CTAs (up to 128 rows x
 // 128 columns): the less of two estimates, in us.
 //   * tiles come in waves of what fits at once; of grouped rows, which are known on the device only, every expert is taken to have the
-//     average, and a tile that it fills half;
+//     average of all rows that the operand has room for, and a tile that it fills half: where a step fills little of a long buffer, as an expert layer made for more
+//     tokens does, the rule plans for rows that are not there (a layer of 32 experts, 7168 and 2048, on 64 tokens: made for 64 185 us, for 4096 213);
 //   * single: a stage of 256 columns of K takes 0.19 us to issue, or its bytes at 112 a ns; a tile at least 0.4 us and 1.6 a 128 rows, in which
 //     the tile in front is stored;
 //   * pair: 0.34 us a stage, and 1.5 in which nothing overlaps the reading of the tile's accumulator;
@@ -110,8 +111,8 @@ template <typename Kernel> cudaError_t Launch(Kernel *kernel, int ctas, int clus
 // 2048 x 4096 x 1024 11.5 / 10.5, 4096 x 4096 x 4096 36 / 29, 8192 x 28672 x 8192 862 / 642; 32 experts, 7168 and 2048, gated and down: 64 rows
 // 67 / 81 and 37 / 54, 3000 94 / 111 and 55 / 66, 5003 106 / 123 and 69 / 76, 8000 138 / 137 and 91 / 88, 16000 234 / 215 and 153 / 142.
 //
-// Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles that there can be fit at once and that is estimated to be
-// faster: exchanging sums takes 0.9 us, 0.2 a CTA and 12 ns a row.  us, alone / 2 / 4 / 8 of them: 1 x 4096 x 14336 15.0 / 10.6 / 9.5 / -,
+// Single CTAs share a tile along K, as clusters of 2, 4 or 8, where the clusters of all tiles that there can be fit at once (by expert: of any split of the operand's
+// rows, so of a few rows only) and that is estimated to be faster: exchanging sums takes 0.9 us, 0.2 a CTA and 12 ns a row.  us, alone / 2 / 4 / 8 of them: 1 x 4096 x 14336 15.0 / 10.6 / 9.5 / -,
 // 16 x 8192 x 28672 28.1 / 24.7 / - / -, 128 x 1024 x 4096 8.4 / 8.5 / 7.0 / 7.1, 16 x 8192 x 3584 6.8 / 7.6 / - / -, 16 x 4096 x 1024 3.8 / 4.5 / 5.2 / -.
 struct Costs { double single, pair; int split; };
 Costs Estimate(int64_t M, int64_t N, int64_t K, int experts, bool glu, int sms, int pairs, const int (&clusters)[3])

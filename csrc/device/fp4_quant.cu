@@ -7,7 +7,7 @@
 //
 // Memory is what bounds it: 2 bytes read and 17/32 written a value (bf16).  A lane takes 16 values (32 of fp8) of a row, two (one) a block
 // of 32, and stays in its columns from row to row, so that neither shared memory nor a second pass nor address arithmetic is in the way.
-// 8192 x 28672 bf16: 97 us, 6.1 TB/s (eight values a lane and addresses by division: 281 us); back to bf16 102.
+// 8192 x 28672 bf16: 99 us, 6.0 TB/s (eight values a lane and addresses by division: 281 us); back to bf16 101.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -17,9 +17,11 @@
 // maximum (redux) and a ballot.  Sums over tokens stay in registers for as long as a warp works, then go to shared memory and, a
 // row for each block, to scratch; they are added up in a fixed order, so results do not depend on which block was first.
 //
-// What bounds it is the latency of a token's chain - maximum after maximum, then exponentials and sums across lanes - and beyond some
-// ten thousand tokens the instructions: us forward with counts and loss / backward, floor by bytes: 4096 x 256 bf16 11.6 / 5.8 (0.4, 0.7), 65003 x 64
-// fp32 34 / 20 (3, 6), 65536 x 256 fp32 70 / 47 (11, 21); 16 x 256 with a bias 6.0.  A token's row is asked for one token ahead (65536 x 256 fp32 backward 62 -> 47).
+// What bounds it beyond some ten thousand tokens is instructions: 65003 x 64 and 65536 x 256 use 84 and 83 % of the issue slots forward, 69 and 71 backward,
+// with HBM at 6 to 24 %; one block of 64 registers a SM keeps two to three warps ready in each cycle.  Below that it is the latency of a token's chain -
+// maximum after maximum, then exponentials and sums across lanes - and the launches: 4096 x 256, one token a warp, 62 and 49 %.
+// us forward with counts and loss / backward, floor by bytes: 4096 x 256 bf16 11.7 / 6.3 (0.4, 0.7), 65003 x 64 fp32 34 / 19 (3, 6), 65536 x 256 fp32
+// 70 / 45 (11, 21); 16 x 256 with a bias 5.9.  A token's row is asked for one token ahead (65536 x 256 fp32 backward 62 -> 47).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -235,7 +235,9 @@ def gemm_fp4(a: Fp4Tensor, b: Fp4Tensor, out: torch.Tensor | None = None) -> tor
 
 
 def gemm_fp4_swiglu(a: Fp4Tensor, gate: Fp4Tensor, up: Fp4Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``silu(a @ gate.T) * (a @ up.T)``, bf16, from the fp32 accumulators of both; rows grouped by expert as in ``gemm_fp4``."""
+    """``silu(a @ gate.T) * (a @ up.T)``, bf16, from the fp32 accumulators of both; rows grouped by expert as in ``gemm_fp4``.
+
+    silu is taken as 0 where its argument is below -87.3, where its magnitude is below 2^-119."""
     if a.__class__ is gate.__class__ is up.__class__ is Fp4Tensor and gate.offsets is up.offsets is None:
         r = _short_swiglu(a.values, a.scales, a.offsets, out, gate.values, gate.scales, up.values, up.scales)
         if r is not None:

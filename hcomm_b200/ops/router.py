@@ -8,7 +8,8 @@
 
 ``gates`` and ``loss`` have gradients with regard to the logits (in reverse mode, once); choices and counts are constants.  With f_e the share of the
 tokens' choices that went to expert e and P_e the tokens' mean probability of it, the loss is ``balance * experts * sum f_e P_e``, which is
-``balance`` where both are even.
+``balance`` where both are even.  A backward pass is captured into a CUDA graph while no eager graph of the same leaves lives, which is torch's rule for
+every operator.
 """
 from __future__ import annotations
 

@@ -18,6 +18,10 @@ from ..ops.router import route
 class ExpertParallelMlp:
     """``combine(gates, down_e(silu(gate_e(x)) * up_e(x)))`` over the ``topk`` experts e of each token; inference only.
 
+    The router's logits are products in bf16 with fp32 sums, rounded to bf16 as ``gemm_bf16`` leaves them: experts whose logits agree in those eight
+    bits are a tie, which the lower index wins.  A program that routes on logits in fp32 calls ``route`` and the exchange itself.
+    Products by expert are planned for the rows that ``max_tokens`` may bring, so a layer made for what a step holds is the faster one.
+
     Weights: router bf16 [experts, hidden]; gate and up [local experts, intermediate, hidden] and down [local experts, hidden,
     intermediate], bf16 (quantised here) or ``Fp4Tensor``; random-initialised N(0, 0.02) unless given.  hidden as ``MoeExchange`` takes it,
     intermediate a multiple of 32.  Creating a layer is a collective call, and so is each forward pass; passes of one layer

@@ -9,7 +9,8 @@ Baseline: the same data movement with separate kernels and NCCL: quantise (PyTor
 all_to_all_single of the counts, of the fp8 rows and of the scales; combine = all_to_all_single of the bf16 rows
 back, un-sort, weighted sum.  Router logits are N(0,1); the top-k experts of a token are the largest logits, the
 gates their softmax.  With ``--intermediate F`` the whole layer as well: router, routing, exchange and the experts' gated
-feed-forward of that width in 4 bits (``parallel.ep.ExpertParallelMlp``), bytes of its weights and arithmetic per second on this rank.  Times are CUDA-event medians with an L2 flush between iterations, maximum over ranks.
+feed-forward of that width in 4 bits (``parallel.ep.ExpertParallelMlp``), bytes of its weights and arithmetic per second on this rank
+(the layer is made for these tokens; one made for more is slower at them).  Times are CUDA-event medians with an L2 flush between iterations, maximum over ranks.
 """
 from __future__ import annotations
 

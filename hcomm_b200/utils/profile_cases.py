@@ -9,6 +9,7 @@
     python -m hcomm_b200.utils.profile_cases moe             MoE dispatch + combine, one rank (256 experts, top-8, hidden 7168)
     python -m hcomm_b200.utils.profile_cases single          kernels of the single-GPU cases: the plain GEMM at five shapes, MoE, a scaled copy (two rounds of eight)
     python -m hcomm_b200.utils.profile_cases experts         routing forward and backward, 4-bit quantisation and products: few rows, one rank's experts, many rows (two rounds of fourteen)
+    python -m hcomm_b200.utils.profile_cases routing         routing with counts and loss and its gradient: 4096 x 256, 65003 x 64, 65536 x 256 (two rounds of nine)
 
 Ranks that share the GPU run inside ONE cooperative launch (kernels that wait for each other are never separate
 launches on a GPU), so each case is a single process a profiler can wrap.  A few launches per kernel, a few hundred
@@ -227,10 +228,22 @@ def case_experts(reps=2):
     assert take_kernel_error() == 0
 
 
+def case_routing(reps=2):
+    """Two rounds of: routing with counts and loss, and its gradient, of 4096 tokens of 256 experts in bf16, 65003 of 64 and 65536 of 256 in fp32."""
+    from ..ops.router import route
+    cases = [(torch.randn(t, e, device="cuda").to(dtype).requires_grad_(), k, renormalize)
+             for t, e, k, dtype, renormalize in ((4096, 256, 8, torch.bfloat16, True), (65003, 64, 6, torch.float32, False), (65536, 256, 8, torch.float32, True))]
+    for _ in range(reps):
+        for logits, topk, renormalize in cases:
+            r = route(logits, topk, renormalize=renormalize, balance=0.01)
+            torch.autograd.grad((r.gates, r.loss), logits, (torch.ones_like(r.gates), torch.ones_like(r.loss)))
+    torch.cuda.synchronize()
+
+
 def main():
     torch.cuda.set_device(0)
     which = sys.argv[1] if len(sys.argv) > 1 else "gemm"
-    {"gemm": case_gemm, "gemm_up": case_gemm_up, "gemm_raster": case_gemm_raster, "fused": case_fused, "fused_pair": case_fused_pair, "allreduce": case_allreduce, "moe": case_moe, "single": case_single, "experts": case_experts}[which]()
+    {"gemm": case_gemm, "gemm_up": case_gemm_up, "gemm_raster": case_gemm_raster, "fused": case_fused, "fused_pair": case_fused_pair, "allreduce": case_allreduce, "moe": case_moe, "single": case_single, "experts": case_experts, "routing": case_routing}[which]()
     print(f"profile case {which}: done", flush=True)
 
 

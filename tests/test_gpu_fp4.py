@@ -521,3 +521,18 @@ def test_gates_far_below_zero(m, n, k, grouped):
     x[:, 40], up[:, 40] = 1.0, 3.0          # a block of their own: up is 3
     out = gemm_fp4_swiglu(quantize_fp4(x), quantize_fp4(huge), quantize_fp4(up[:2]))
     assert (out[:, 0] == float("inf")).all() and torch.isnan(out[:, 1]).all()          # inf 1 3; -inf 0
+
+
+def test_the_deepest_product():
+    """As deep as a product may be: a row of 2^31 - 288 columns by itself, nothing but its first and last blocks filled."""
+    from hcomm_b200.ops.fp4 import Fp4Tensor, gemm_fp4, gemm_fp4_swiglu, take_kernel_error
+    torch.cuda.set_device(0)
+    k = 2 ** 31 - 288
+    values = torch.zeros(1, k // 2, device="cuda", dtype=torch.uint8)
+    values[0, :16], values[0, -16:] = 0x22, 0x44            # 32 ones, 32 twos
+    q = Fp4Tensor(values, torch.full((-(-k // 128), 512), 127, device="cuda", dtype=torch.uint8))         # 10 GB
+    assert gemm_fp4(q, q).item() == 32 + 4 * 32
+    assert gemm_fp4_swiglu(q, q, q).item() == 160 * 160
+    assert take_kernel_error() == 0
+    del q, values
+    torch.cuda.empty_cache()

@@ -71,13 +71,13 @@ class ExpertParallelMlp:
 
     def _check(self, x, out):
         """Before anything is queued: the exchange behind is a collective call, and writes where it is told to."""
-        hidden = self.router.shape[1]
-        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != hidden or not x.is_contiguous() or x.device != self.router.device:
-            raise ValueError(f"x must be contiguous bfloat16 [tokens, {hidden}] on {self.router.device}")
-        if x.shape[0] > self.moe.max_tokens:
-            raise ValueError(f"{x.shape[0]} tokens: the layer was made for {self.moe.max_tokens}")
-        if out is not None and (out.dtype != torch.bfloat16 or out.shape != x.shape or not out.is_contiguous() or out.device != x.device):
-            raise ValueError(f"out must be contiguous bfloat16 {list(x.shape)} on {x.device}")
+        shape, device, kind = x.shape, x.device, torch.bfloat16
+        if len(shape) != 2 or shape[1] != self.moe.hidden or x.dtype is not kind or not x.is_contiguous() or device != self.router.device:
+            raise ValueError(f"x must be contiguous bfloat16 [tokens, {self.moe.hidden}] on {self.router.device}")
+        if shape[0] > self.moe.max_tokens:
+            raise ValueError(f"{shape[0]} tokens: the layer was made for {self.moe.max_tokens}")
+        if out is not None and (out.dtype is not kind or out.shape != shape or not out.is_contiguous() or out.device != device):
+            raise ValueError(f"out must be contiguous bfloat16 {list(shape)} on {device}")
 
     def destroy(self):
         self.moe.destroy()

@@ -10,7 +10,7 @@ from hcomm_b200.parallel.ep import ExpertParallelMlp
 def layer():
     made = ExpertParallelMlp.__new__(ExpertParallelMlp)
     made.router = torch.zeros(8, 512, dtype=torch.bfloat16)
-    made.moe = SimpleNamespace(max_tokens=16)
+    made.moe = SimpleNamespace(hidden=512, max_tokens=16)
     return made
 
 

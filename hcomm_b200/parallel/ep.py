@@ -76,8 +76,8 @@ class ExpertParallelMlp:
             raise ValueError(f"x must be contiguous bfloat16 [tokens, {self.moe.hidden}] on {self.router.device}")
         if shape[0] > self.moe.max_tokens:
             raise ValueError(f"{shape[0]} tokens: the layer was made for {self.moe.max_tokens}")
-        if out is not None and (out.dtype is not kind or out.shape != shape or not out.is_contiguous() or out.device != device):
-            raise ValueError(f"out must be contiguous bfloat16 {list(shape)} on {device}")
+        if out is not None and (out.dtype is not kind or out.dim() != 2 or out.shape[0] < shape[0] or out.shape[1] != shape[1] or not out.is_contiguous() or out.device != device):
+            raise ValueError(f"out must be contiguous bfloat16 {list(shape)} on {device}, or have more rows, which are left as they are")
 
     def destroy(self):
         self.moe.destroy()

@@ -26,8 +26,13 @@ def test_tokens(x):
 
 
 @pytest.mark.parametrize("x", [X, X[:0]])
-@pytest.mark.parametrize("out", [torch.zeros(4, 512), torch.zeros(3, 512, dtype=BF16), torch.zeros(5, 512, dtype=BF16), torch.zeros(4, 256, dtype=BF16), torch.zeros(2048, dtype=BF16),
+@pytest.mark.parametrize("out", [torch.zeros(4, 512), torch.zeros(4, 256, dtype=BF16), torch.zeros(2048, dtype=BF16),
                                  torch.zeros(512, 4, dtype=BF16).t(), torch.zeros(4, 1024, dtype=BF16)[:, :512], X.to("meta")])
 def test_results(x, out):
     with pytest.raises(ValueError, match="out"):
         layer()(x, out)
+
+
+def test_a_result_of_too_few_rows():
+    with pytest.raises(ValueError, match="out"):
+        layer()(X, torch.zeros(3, 512, dtype=BF16))

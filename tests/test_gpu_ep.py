@@ -226,3 +226,16 @@ def test_combine_carries_gates_that_are_no_numbers_where_it_is_asked_to(through_
     finally:
         moe.destroy()
         comm.destroy()
+
+
+def test_a_result_with_more_rows_than_tokens():
+    g = gen(95)
+    comms, (layer,) = make(1, experts=8, topk=2, hidden=512, intermediate=64, max_tokens=20)
+    try:
+        x = torch.randn(20, 512, device="cuda", generator=g).to(torch.bfloat16)
+        want = layer(x).clone()
+        for n in (20, 7, 0):
+            out = torch.full((20, 512), 5.0, device="cuda", dtype=torch.bfloat16)
+            assert layer(x[:n], out) is out and torch.equal(out[:n], want[:n]) and (out[n:] == 5).all()
+    finally:
+        end(comms, [layer])
